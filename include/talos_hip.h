@@ -28,6 +28,8 @@ extern "C" {
 #endif
 
 typedef void* talos_stream_t;
+/* A bfloat16 value's bits (the high half of the fp32 that it stands for). */
+typedef uint16_t talos_bf16;
 
 enum talos_status {
   TALOS_OK = 0,
@@ -144,6 +146,27 @@ int talos_rmsnorm_fwd_f32(int rows, int dim, float eps, const float* x, const fl
 int talos_rmsnorm_bwd_f32(int rows, int dim, const float* x, const float* w, const float* rstd, const float* dy,
                           float beta_dx, float* dx, float beta_dw, float* dw, talos_stream_t stream);
 
+/* Layer norm over the last dimension, beside the RMSNorm above (no counterpart among the reference's
+ * modules): y = (x - mean) * rstd * w + b with the row's mean and biased variance, rstd =
+ * 1 / sqrt(var + eps). x and y are contiguous [rows, dim] at any element alignment; w [dim] and b
+ * [dim] (b may be NULL: no bias) are fp32. Saves mean[rows] and rstd[rows] for the backward (either
+ * may be NULL). The _bf16 entries take bf16 x, y, dy and dx; statistics, sums and the parameters'
+ * gradients are fp32, and a bf16 result is rounded once. dim <= 2^26. y may be x. */
+int talos_layernorm_fwd_f32(int rows, int dim, float eps, const float* x, const float* w, const float* b, float* y,
+                            float* mean, float* rstd, talos_stream_t stream);
+int talos_layernorm_fwd_bf16(int rows, int dim, float eps, const talos_bf16* x, const float* w, const float* b,
+                             talos_bf16* y, float* mean, float* rstd, talos_stream_t stream);
+/* Its backward: with xh = (x - mean) * rstd and h = dy * w, dx = beta_dx dx + rstd * (h - mean(h) -
+ * xh * mean(h * xh)), dw = beta_dw dw + sum_rows dy * xh, db = beta_dw db + sum_rows dy (partial sums
+ * added in f64, deterministic). dw and db may each be NULL; dx may be dy. Scratch: up to 512 partial
+ * rows of 2 dim floats (talos_workspace_bind). */
+int talos_layernorm_bwd_f32(int rows, int dim, const float* x, const float* w, const float* mean, const float* rstd,
+                            const float* dy, float beta_dx, float* dx, float beta_dw, float* dw, float* db,
+                            talos_stream_t stream);
+int talos_layernorm_bwd_bf16(int rows, int dim, const talos_bf16* x, const float* w, const float* mean,
+                             const float* rstd, const talos_bf16* dy, float beta_dx, talos_bf16* dx, float beta_dw,
+                             float* dw, float* db, talos_stream_t stream);
+
 /* Row softmax (transformer.rs:1074-1096) with max subtraction. causal != 0 adds the
  * causal mask: row r is query q = r mod cols, keys j > q get probability exactly 0
  * (extension; the reference has no mask). */
@@ -190,6 +213,19 @@ int talos_attn_bwd_noalloc_f32(int batch, int seq, int heads, int qk_dim, int v_
                                const float* q, int ld_q, const float* k, int ld_k, const float* v, int ld_v,
                                const float* o, int ld_o, const float* lse, const float* dout, int ld_do, float* dq,
                                int ld_dq, float* dk, int ld_dk, float* dv, int ld_dv, talos_stream_t stream);
+
+/* A learned relative position bias by buckets: bias[h, d + M] = table[bucket(d), h] for the distances
+ * d = -M .. M (key position - query position, M = max_distance). Of a side's S buckets (num_buckets, or
+ * half of them where bidirectional = 1, the second half for keys after the query) the first E = S / 2
+ * hold one distance each and the rest split E .. M evenly by logarithm: bucket(n) = n for n < E, else
+ * min(S - 1, E + floor((S - E) ln(n / E) / ln(M / E) + 1e-9)) (f64), n = |d|, or max(0, -d) where
+ * bidirectional = 0. table [num_buckets, heads], bias [heads, 2 M + 1]; buckets (int32 [2 M + 1]) may
+ * be NULL. M > E, num_buckets <= 4096, M <= 2^20. */
+int talos_relpos_bias_fwd_f32(int num_buckets, int heads, int max_distance, int bidirectional, const float* table,
+                              float* bias, int32_t* buckets, talos_stream_t stream);
+/* dtable[b, h] = beta dtable[b, h] + the sum of dbias[h, .] over the bucket's distances (f64, fixed order). */
+int talos_relpos_bias_bwd_f32(int num_buckets, int heads, int max_distance, int bidirectional, const float* dbias,
+                              float beta, float* dtable, talos_stream_t stream);
 
 /* Element-wise ops of the tape (autograd.rs:356-792, 1606-1862). */
 enum talos_unary_op {
@@ -430,6 +466,46 @@ int talos_ppo_head_loss_bwd_f32(int n, int n_actions, float clip_eps, float valu
                                 const float* logits, const float* values, const int32_t* actions, const float* adv,
                                 const float* ret, const float* old_logp, float* dlogits, float* dvalues, float* loss,
                                 talos_stream_t stream);
+/* The clipped policy loss with a KL term over wide rows of logits (a token's vocabulary, a large action
+ * set), beside talos_ppo_head_loss_* above. Row t of logits [rows, vocab] (row stride ld_logits) took
+ * action a_t:
+ *   logp = log_softmax(logits)[a],  ratio = exp(logp - old_logp),
+ *   gain = min(ratio adv, clip(ratio, 1 - clip_low, 1 + clip_high) adv)   (ties take the clipped one),
+ *   kl   = exp(ref_logp - logp) - (ref_logp - logp) - 1,
+ *   loss = sum_t weight_t (kl_coef kl_t - gain_t)
+ * ref_logp may be NULL (no KL term, kl_coef 0); weight may be NULL: 1 / rows each. A row of weight 0 is
+ * padding: its logits and scalars are not used, its logp and gradient are 0. A logit of -infinity is an
+ * action that cannot be taken (the taken one must be finite). An action outside [0, vocab) makes the
+ * loss NaN, with a zero gradient. loss (device float[1]), logp (float[rows]) and stats (device
+ * double[TALOS_POLICY_NSTATS], sums over the rows of non-zero weight, added into when
+ * stats_accumulate != 0) may each be NULL, the forward's not all. vocab <= 2^26. */
+enum talos_policy_stat {
+  TALOS_POLICY_STAT_KL = 0,      /* (ratio - 1) - log ratio against the rollout's policy, as TALOS_PPO_STAT_KL */
+  TALOS_POLICY_STAT_POLICY = 1,  /* gain */
+  TALOS_POLICY_STAT_REF_KL = 2,  /* kl */
+  TALOS_POLICY_STAT_CLIPPED = 3, /* rows whose ratio is clipped */
+  TALOS_POLICY_STAT_COUNT = 4,
+  TALOS_POLICY_NSTATS = 5
+};
+int talos_policy_loss_fwd_f32(int rows, int vocab, float clip_low, float clip_high, float kl_coef, const float* logits,
+                              long long ld_logits, const int32_t* actions, const float* adv, const float* old_logp,
+                              const float* ref_logp, const float* weight, float* loss, float* logp, double* stats,
+                              int stats_accumulate, talos_stream_t stream);
+int talos_policy_loss_fwd_bf16(int rows, int vocab, float clip_low, float clip_high, float kl_coef,
+                               const talos_bf16* logits, long long ld_logits, const int32_t* actions, const float* adv,
+                               const float* old_logp, const float* ref_logp, const float* weight, float* loss,
+                               float* logp, double* stats, int stats_accumulate, talos_stream_t stream);
+/* The loss and its gradient in one pass over the logits: dlogits [rows, vocab] (row stride ld_dlogits) is
+ * overwritten; it may be the logits' own buffer with the same stride. Columns past vocab are left. */
+int talos_policy_loss_bwd_f32(int rows, int vocab, float clip_low, float clip_high, float kl_coef, const float* logits,
+                              long long ld_logits, const int32_t* actions, const float* adv, const float* old_logp,
+                              const float* ref_logp, const float* weight, float* dlogits, long long ld_dlogits,
+                              float* loss, float* logp, double* stats, int stats_accumulate, talos_stream_t stream);
+int talos_policy_loss_bwd_bf16(int rows, int vocab, float clip_low, float clip_high, float kl_coef,
+                               const talos_bf16* logits, long long ld_logits, const int32_t* actions, const float* adv,
+                               const float* old_logp, const float* ref_logp, const float* weight, talos_bf16* dlogits,
+                               long long ld_dlogits, float* loss, float* logp, double* stats, int stats_accumulate,
+                               talos_stream_t stream);
 /* Forward only for n samples with optional lengths (the rollout's log-probs and values). */
 int talos_ppo_forward_n_f32(talos_plan plan, int n, const float* params, const float* states,
                             const int32_t* lengths, float* logits, float* values, talos_stream_t stream);

@@ -75,6 +75,18 @@ class MlaCfg(ctypes.Structure):
 
 PREC_FP32, PREC_BF16 = 0, 1
 
+
+POLICY_NSTATS = 5
+POLICY_STAT_KL, POLICY_STAT_POLICY, POLICY_STAT_REF_KL, POLICY_STAT_CLIPPED, POLICY_STAT_COUNT = range(5)
+
+# operators with an fp32 and a bf16 form of the same arguments
+_TYPED_SIGS = {
+    "talos_layernorm_fwd": [_i, _i, _f, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "talos_layernorm_bwd": [_i, _i, _vp, _vp, _vp, _vp, _vp, _f, _vp, _f, _vp, _vp, _vp],
+    "talos_policy_loss_fwd": [_i, _i, _f, _f, _f, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp],
+    "talos_policy_loss_bwd": [_i, _i, _f, _f, _f, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp, _vp, _vp, _i, _vp],
+}
+
 # name -> argtypes (restype int unless listed in _RESTYPE)
 _SIGS = {
     "talos_last_error": [],
@@ -160,9 +172,12 @@ _SIGS = {
     "talos_ppo_checkpoint_decode": [ctypes.POINTER(PpoCfg), _vp, _sz, _i, _vp],
     "talos_ppo_checkpoint_save": [ctypes.POINTER(PpoCfg), _vp, _i, ctypes.c_char_p],
     "talos_ppo_checkpoint_load": [ctypes.POINTER(PpoCfg), ctypes.c_char_p, _vp],
+    "talos_relpos_bias_fwd_f32": [_i, _i, _i, _i, _vp, _vp, _vp, _vp],
+    "talos_relpos_bias_bwd_f32": [_i, _i, _i, _i, _vp, _f, _vp, _vp],
     "talos_plan_profiler": [_vp, ctypes.POINTER(_vp)],
     "talos_profiler_enable": [_vp, _i, ctypes.c_char_p],
     "talos_profiler_read": [_vp, _vp, _i, ctypes.POINTER(_i)],
+    **{f"{name}_{t}": args for name, args in _TYPED_SIGS.items() for t in ("f32", "bf16")},
 }
 
 
