@@ -214,6 +214,66 @@ int talos_attn_bwd_noalloc_f32(int batch, int seq, int heads, int qk_dim, int v_
                                const float* o, int ld_o, const float* lse, const float* dout, int ld_do, float* dq,
                                int ld_dq, float* dk, int ld_dk, float* dv, int ld_dv, talos_stream_t stream);
 
+/* Grouped-query attention of any length, beside the fused attention above (which holds a sequence of
+ * at most 256 tokens on its chip and has as many key heads as query heads): heads / kv_heads query
+ * heads in a row share a key / value head, queries and keys have lengths of their own, each sample may
+ * be shorter than the padded length, and a bias by distance may be added to the scores. The
+ * probabilities are never stored: one pass over the keys with a running maximum and sum, and the
+ * backward forms them again from lse.
+ *
+ * q [batch, q_len, heads, qk_dim], k [batch, k_len, kv_heads, qk_dim], v [batch, k_len, kv_heads, v_dim],
+ * o [batch, q_len, heads, v_dim], with row strides ld_* (elements between consecutive tokens; sample b
+ * begins at row b * q_len or b * k_len), at any element alignment; lse[batch, heads, q_len] is fp32.
+ * q_lens, k_lens: device int32[batch] (NULL: all q_len, k_len), clamped to [0, q_len] and [0, k_len].
+ * Rows past a sample's length are not read (they may hold anything). The queries and keys of a sample
+ * end together: query i stands at position i + k_lens[b] - q_lens[b], so the same call serves whole
+ * sequences, a chunk of new tokens or a single one after a cache, and a causal query sees the keys j
+ * <= its position.
+ *   s_ij = scale q_i . k_j + bias[h, clamp(j - position_i, -M, M) + M],   o_i = sum_j softmax_j(s_i) v_j,
+ *   lse_i = ln sum_j exp(s_ij)
+ * bias: fp32 [heads, 2 M + 1], M = max_distance, or NULL (talos_relpos_bias_fwd_f32 makes one from a
+ * table by buckets). A query that sees no key, and every row past q_lens[b], gets o = 0 and lse =
+ * -infinity.
+ *
+ * talos_gqa_fwd_f32 / _bwd_f32 take fp32 tensors and products of three-piece bf16 splits (fp32
+ * accuracy, as talos_gemm_f32; values past 3.39e38 give NaN, and bits of a product below 2^-133 are
+ * lost); the _bf16 entries take bf16 q, k, v, o and their gradients, with fp32 scores, softmax and
+ * accumulators, the probabilities and their gradients rounded to bf16 as operands.
+ * qk_dim, v_dim <= 128. batch * heads <= 65535 and a sample's stride is not limited to 32 bits. */
+typedef struct talos_gqa_cfg {
+  int batch;
+  int q_len;
+  int k_len;
+  int heads;
+  int kv_heads;     /* divides heads */
+  int qk_dim;
+  int v_dim;
+  int causal;
+  int max_distance; /* M of the bias; ignored without one */
+  float scale;
+} talos_gqa_cfg;
+int talos_gqa_fwd_f32(const talos_gqa_cfg* cfg, const int32_t* q_lens, const int32_t* k_lens, const float* bias,
+                      const float* q, long long ld_q, const float* k, long long ld_k, const float* v, long long ld_v,
+                      float* o, long long ld_o, float* lse, talos_stream_t stream);
+int talos_gqa_fwd_bf16(const talos_gqa_cfg* cfg, const int32_t* q_lens, const int32_t* k_lens, const float* bias,
+                       const talos_bf16* q, long long ld_q, const talos_bf16* k, long long ld_k, const talos_bf16* v,
+                       long long ld_v, talos_bf16* o, long long ld_o, float* lse, talos_stream_t stream);
+/* Its backward from o and lse of the forward: dq, dk, dv are overwritten (zero past the lengths; the
+ * heads of a group add into their shared key head), and dbias = beta_bias dbias + the scores'
+ * gradients summed by distance, when bias is given and dbias is not NULL (M <= 512). Every sum has a
+ * fixed order: no atomics, the same bits on every call. Scratch (talos_workspace_bind): the rows'
+ * D = rowsum(dout * o) and, where the work is split, partial sums. */
+int talos_gqa_bwd_f32(const talos_gqa_cfg* cfg, const int32_t* q_lens, const int32_t* k_lens, const float* bias,
+                      const float* q, long long ld_q, const float* k, long long ld_k, const float* v, long long ld_v,
+                      const float* o, long long ld_o, const float* lse, const float* dout, long long ld_do, float* dq,
+                      long long ld_dq, float* dk, long long ld_dk, float* dv, long long ld_dv, float beta_bias,
+                      float* dbias, talos_stream_t stream);
+int talos_gqa_bwd_bf16(const talos_gqa_cfg* cfg, const int32_t* q_lens, const int32_t* k_lens, const float* bias,
+                       const talos_bf16* q, long long ld_q, const talos_bf16* k, long long ld_k, const talos_bf16* v,
+                       long long ld_v, const talos_bf16* o, long long ld_o, const float* lse, const talos_bf16* dout,
+                       long long ld_do, talos_bf16* dq, long long ld_dq, talos_bf16* dk, long long ld_dk,
+                       talos_bf16* dv, long long ld_dv, float beta_bias, float* dbias, talos_stream_t stream);
+
 /* A learned relative position bias by buckets: bias[h, d + M] = table[bucket(d), h] for the distances
  * d = -M .. M (key position - query position, M = max_distance). Of a side's S buckets (num_buckets, or
  * half of them where bidirectional = 1, the second half for keys after the query) the first E = S / 2

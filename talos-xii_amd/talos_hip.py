@@ -76,6 +76,11 @@ class MlaCfg(ctypes.Structure):
 PREC_FP32, PREC_BF16 = 0, 1
 
 
+class GqaCfg(ctypes.Structure):
+    _fields_ = [("batch", _i), ("q_len", _i), ("k_len", _i), ("heads", _i), ("kv_heads", _i), ("qk_dim", _i),
+                ("v_dim", _i), ("causal", _i), ("max_distance", _i), ("scale", _f)]
+
+
 POLICY_NSTATS = 5
 POLICY_STAT_KL, POLICY_STAT_POLICY, POLICY_STAT_REF_KL, POLICY_STAT_CLIPPED, POLICY_STAT_COUNT = range(5)
 
@@ -83,6 +88,9 @@ POLICY_STAT_KL, POLICY_STAT_POLICY, POLICY_STAT_REF_KL, POLICY_STAT_CLIPPED, POL
 _TYPED_SIGS = {
     "talos_layernorm_fwd": [_i, _i, _f, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "talos_layernorm_bwd": [_i, _i, _vp, _vp, _vp, _vp, _vp, _f, _vp, _f, _vp, _vp, _vp],
+    "talos_gqa_fwd": [ctypes.POINTER(GqaCfg), _vp, _vp, _vp, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp],
+    "talos_gqa_bwd": [ctypes.POINTER(GqaCfg), _vp, _vp, _vp, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _ll,
+                      _vp, _ll, _vp, _ll, _vp, _ll, _f, _vp, _vp],
     "talos_policy_loss_fwd": [_i, _i, _f, _f, _f, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp],
     "talos_policy_loss_bwd": [_i, _i, _f, _f, _f, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp, _vp, _vp, _i, _vp],
 }
