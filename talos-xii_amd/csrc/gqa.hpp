@@ -41,6 +41,9 @@ struct GqaArgs {
   float* dbias_part;      // [B][H][tiles][splits_q][2 M + 1]
 };
 
+// the wave's number, known to the compiler to be one for all its lanes
+__device__ __forceinline__ int gq_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 template <typename T>
 constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
 
@@ -167,29 +170,43 @@ __device__ __forceinline__ Frag<NP> gq_frag_acc(const float* f) {
   }
   return r;
 }
-// row r, chunk c of a tile whose planes are PL elements apart
+// A lane's places in a tile, in bytes from its start. Row operands read row l32 (of a block of 32) and chunk 2 s + h;
+// transposing reads read 4 x 16 blocks by groups of 16 lanes: lane 4 a + j of group g reads row 4 (g / 2) + a (and 8
+// further) from column 16 (g % 2) + 4 j on, and receives one column of the four rows. Steps along the columns flip
+// address bits above the lane's own (the chunks are permuted by XOR), steps along the rows are constants.
+template <int D>
+struct GqaLane {
+  uint32_t row, tr;
+  __device__ __forceinline__ GqaLane() {
+    const int lane = threadIdx.x & 63, g = lane >> 4, a = (lane >> 2) & 3, j = lane & 3;
+    row = 2 * gq_at<D>(lane & 31, lane >> 5);
+    tr = 2 * (gq_at<D>(4 * (g >> 1) + a, 2 * (g & 1) + (j >> 1)) + 4 * (j & 1));
+  }
+  // makes the compiler form the addresses anew (an instruction each) where it would keep dozens in registers
+  __device__ __forceinline__ void renew() { asm volatile("" : "+v"(row), "+v"(tr)); }
+};
+// chunk 2 s + h of row rb + l32 (rb a multiple of 32) of a tile whose planes are PL elements apart
 template <int NP, int D, int PL>
-__device__ __forceinline__ Frag<NP> gq_frag_row(const uint16_t* tile, int r, int c) {
+__device__ __forceinline__ Frag<NP> gq_frag_row(const uint16_t* tile, const GqaLane<D>& ln, int rb, int s) {
+  const char* at = reinterpret_cast<const char*>(tile) + (ln.row ^ (uint32_t)(32 * s)) + 2 * rb * D;
   Frag<NP> f;
 #pragma unroll
   for (int i = 0; i < NP; ++i)
-    f.p[i] = __builtin_bit_cast(gq_bf16x8, *reinterpret_cast<const uint4*>(tile + i * PL + gq_at<D>(r, c)));
+    f.p[i] = __builtin_bit_cast(gq_bf16x8, *reinterpret_cast<const uint4*>(at + 2 * i * PL));
   return f;
 }
-// The transposed tile's fragment for column block c0 (a multiple of 32) and rows r0 + 4 h + 0..3 and r0 + 8 +
-// 4 h + 0..3 (r0 a multiple of 16): lane (l32, h) gets them of column c0 + l32. A group of 16 lanes reads a 4 x
-// 16 block: lane 4 a + j the four values of row a from column 4 j on, and receives column l of the four rows.
+// The transposed tile's fragment for column block 32 ob and rows r0 + 4 h + 0..3 and r0 + 8 + 4 h + 0..3 (r0 a multiple
+// of 16): lane (l32, h) gets them of column 32 ob + l32. Rows 8 further have the permutation's bit 1 flipped.
 template <int NP, int D, int PL>
-__device__ __forceinline__ Frag<NP> gq_frag_tr(const uint16_t* tile, int r0, int c0, int lane) {
+__device__ __forceinline__ Frag<NP> gq_frag_tr(const uint16_t* tile, const GqaLane<D>& ln, int r0, int ob) {
   typedef __attribute__((address_space(3))) gq_s16x4* lds4;
-  const int g = lane >> 4, a = (lane >> 2) & 3, j = lane & 3;
-  const int r = r0 + 4 * (g >> 1) + a, ch = c0 / 8 + 2 * (g & 1) + (j >> 1);
-  const int lo = gq_at<D>(r, ch) + 4 * (j & 1), hi = gq_at<D>(r + 8, ch) + 4 * (j & 1);
+  const char* lo = reinterpret_cast<const char*>(tile) + (ln.tr ^ (uint32_t)(64 * ob)) + 2 * r0 * D;
+  const char* hi = reinterpret_cast<const char*>(tile) + (ln.tr ^ (uint32_t)(64 * ob + 32)) + 2 * (r0 + 8) * D;
   Frag<NP> f;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(tile + i * PL + lo)));
-    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(tile + i * PL + hi)));
+    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(lo + 2 * i * PL)));
+    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(hi + 2 * i * PL)));
     f.p[i] = __builtin_bit_cast(gq_bf16x8, make_uint4(x.x, x.y, y.x, y.y));
   }
   return f;
@@ -213,6 +230,19 @@ __device__ __forceinline__ gq_f32x16 gq_mfma_small(const Frag<3>& a, const Frag<
   return gq_mfma(a.p[1], b.p[0], c);
 }
 
+// An accumulator whose every column holds v of its row, for lane l32's v of row l32: one product of v's three bf16
+// pieces with ones. (A row's value in each of 16 registers would be four 16-byte LDS reads a lane.)
+__device__ __forceinline__ gq_f32x16 gq_rows(float v, int h) {
+  const uint32_t a = bf16_round2(v, 0.f) & 0xffffu;
+  v -= __uint_as_float(a << 16);
+  const uint32_t b = bf16_round2(v, 0.f) & 0xffffu;
+  v -= __uint_as_float(b << 16);
+  const uint32_t c = bf16_round2(v, 0.f) & 0xffffu;
+  const uint4 x = h ? make_uint4(0, 0, 0, 0) : make_uint4(a | b << 16, c, 0, 0);
+  const uint4 one = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+  return gq_mfma(__builtin_bit_cast(gq_bf16x8, x), __builtin_bit_cast(gq_bf16x8, one), gq_zero());
+}
+
 // Accumulator row of register r in lane half h (the column is lane % 32).
 __device__ __forceinline__ constexpr int gq_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
@@ -232,8 +262,8 @@ struct GqaSample {
 };
 __device__ __forceinline__ GqaSample gq_sample(const GqaArgs& a, int b) {
   GqaSample s;
-  s.ql = a.qlens ? min(max(a.qlens[b], 0), a.Sq) : a.Sq;
-  s.kl = a.klens ? min(max(a.klens[b], 0), a.Sk) : a.Sk;
+  s.ql = a.qlens ? __builtin_amdgcn_readfirstlane(min(max(a.qlens[b], 0), a.Sq)) : a.Sq;
+  s.kl = a.klens ? __builtin_amdgcn_readfirstlane(min(max(a.klens[b], 0), a.Sk)) : a.Sk;
   s.off = s.kl - s.ql;
   return s;
 }
@@ -294,6 +324,72 @@ struct GqaTile {
     }
   }
 };
+
+// The same for a bf16 tile whose rows are D values wide and 16-byte aligned, straight from memory into LDS
+// (global_load_lds_dwordx4: lane i's 16 bytes go to the wave's LDS address + 16 i). No registers hold the tile and no
+// LDS stores are issued. An instruction fills 64 chunks of LDS, 512 / D rows, so the permutation of chunks is made on
+// the memory side: each lane fetches the chunk that belongs at its place, the same one for every instruction (the rows
+// of a lane differ by multiples of 16). Rows from `rows` on are filled with the last valid one: scores against it are
+// masked and probabilities of it are zero, as they are for the zero rows above.
+// Issued from inline assembly, so that the compiler does not wait for all of them before every LDS read that follows;
+// gq_dma_wait() and a barrier publish them. Other waits of the compiler's only get stronger by them.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void gq_dma16(const void* base, uint32_t offset, const void* lds) {
+  const uint32_t to =
+      __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds);
+  const uint64_t at = (uint64_t)base;
+  const uint64_t from = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+// waits until at most N of the wave's memory instructions are in flight (those issued last)
+template <int N = 0>
+__device__ __forceinline__ void gq_dma_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// the wave's LDS reads have arrived: what they read may be overwritten
+__device__ __forceinline__ void gq_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// W = 4: the workgroup's waves fetch a tile together. W = 1: a wave fetches a tile of its own (the rows of a lane are then
+// fewer than 16 apart, and the chunk it fetches changes with the instruction).
+template <int D, int NR, int W = 4>
+struct GqaDma {
+  static constexpr int CH = D / 8, RPI = 64 / CH, PER = NR * CH / (64 * W);  // rows an instruction, instructions a wave
+  static_assert(NR * CH % (64 * W) == 0 && (W == 1 || W * RPI % 16 == 0), "whole instructions, rows 16 apart");
+  int row;                 // this lane's row of the first instruction
+  uint32_t offset, chunk;  // in bytes, from the tile's first row: that row's, and the chunk's in it
+  __device__ __forceinline__ void init(long long ld) {
+    const int lane = threadIdx.x & 63;
+    row = (W == 1 ? 0 : gq_wave() * RPI) + lane / CH;
+    const int place = gq_at<D>(row, 0) / 8 % CH;  // where chunk 0 of the row stands: the row's permutation
+    offset = (uint32_t)(row * ld) * 2;
+    chunk = 16 * ((lane % CH) ^ place);
+  }
+  // rows row0 .. row0 + NR - 1 of base (row stride ld), of which `rows` exist (row0 < rows)
+  __device__ __forceinline__ void issue(const Bf16* base, long long ld, int row0, int rows, uint16_t* tile) const {
+    constexpr int kTurn = W == 1 && D == 128 ? 1 : W == 1 && D == 64 ? 2 : 0;  // a step of RPI rows in the permutation
+    const int wv = W == 1 ? 0 : gq_wave();
+    if (row0 + NR <= rows) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        gq_dma16(base + (row0 + W * RPI * i) * ld, offset + (chunk ^ (16u * (kTurn * i & 3))), tile + (W * i + wv) * 512);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int over = max(0, row0 + row + W * RPI * i - (rows - 1));  // rows past the last
+        gq_dma16(base + row0 * ld, offset + (chunk ^ (16u * (kTurn * i & 3))) + (uint32_t)((W * RPI * i - over) * ld) * 2,
+                 tile + (W * i + wv) * 512);
+      }
+    }
+  }
+};
+// whether a tensor's rows can be fetched so: ld counted in values
+inline bool gq_dma_fits(const void* p, long long ld) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && ld < (1 << 22);
+}
 
 // Four consecutive values of a row from column d on, n columns in all.
 template <typename T>

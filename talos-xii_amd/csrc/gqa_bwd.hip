@@ -18,10 +18,12 @@
 // product on the K tile's fragments in hand) and subtracts R times it; the dK / dV kernel, which runs after it, gets D' + R.
 //
 // The bias gradient belongs to the second kernel, where one head is at work: a block of 32 keys by 32 queries spans 63
-// distances. Blocks at least M away add into one register a lane; nearer ones add each value to an LDS array by
-// distance, one array for each half of each wave, so the 32 lanes of a half always hit different words: no two
-// additions meet, and the order is the program's. The arrays are folded once a head.
+// distances. Blocks at least M away add into one register a lane; nearer ones sum their diagonals in registers
+// (diagonals() below) and add them, one lane a distance, to an array by distance in LDS that is the wave's own: no two
+// additions meet, and the order is the program's. The four arrays are folded once a head. (Sixteen LDS float atomics a
+// block, each lane its values, cost 224 cycles apiece: 127 us of 322 at 2 x 2048 tokens, 16 heads, d 64, M 128.)
 #include <algorithm>
+#include <type_traits>
 
 #include "gqa.hpp"
 
@@ -35,12 +37,17 @@ struct DqShape {
   static constexpr size_t lds = (size_t)NBUF * BUF * 2;
 };
 
-template <typename T, int D, int NK, int NBUF, int BIAS>
-__global__ __launch_bounds__(256) void gqa_dq_kernel(GqaArgs a) {
+// waves a SIMD that the kernels are compiled for, as in the forward
+template <typename T, int D, bool DMA>
+constexpr int kBwdWaves = D == 128 ? (DMA ? 2 : 1) : sizeof(T) == 4 && D > 32 ? 1 : 2;
+
+// BIAS, DMA: as in the forward
+template <typename T, int D, int NK, int NBUF, bool BIAS, bool DMA>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T, D, DMA>))) void gqa_dq_kernel(GqaArgs a) {
   using S = DqShape<T, D, NK, NBUF>;
   constexpr int NP = S::NP, KS = D / 16, OB = D / 32, KB = NK / 32, PL = NK * D;
   extern __shared__ __align__(16) uint16_t lds[];
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, wv = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, wv = gq_wave();
   const GqaItem it = gq_item(a, true);
   const GqaSample sm = gq_sample(a, it.b);
   const int G = a.G;
@@ -58,10 +65,20 @@ __global__ __launch_bounds__(256) void gqa_dq_kernel(GqaArgs a) {
 
   const T* kbase = static_cast<const T*>(a.k) + (long long)it.b * a.Sk * a.ldk + (long long)it.kvh * a.dk;
   const T* vbase = static_cast<const T*>(a.v) + (long long)it.b * a.Sk * a.ldv + (long long)it.kvh * a.dv;
-  GqaTile<T, D, NK> kt, vt;
+  std::conditional_t<DMA, GqaDma<D, NK>, GqaTile<T, D, NK>> kt, vt;
+  if constexpr (DMA) {
+    kt.init(a.ldk);
+    vt.init(a.ldv);
+  }
   if (t_beg < t_end) {
-    kt.fetch(kbase, a.ldk, t_beg * NK, sm.kl, a.dk);
-    vt.fetch(vbase, a.ldv, t_beg * NK, sm.kl, a.dv);
+    if constexpr (DMA) {
+      uint16_t* buf = lds + (t_beg & 1) * S::BUF;
+      kt.issue(kbase, a.ldk, t_beg * NK, sm.kl, buf);
+      vt.issue(vbase, a.ldv, t_beg * NK, sm.kl, buf + PL);
+    } else {
+      kt.fetch(kbase, a.ldk, t_beg * NK, sm.kl, a.dk);
+      vt.fetch(vbase, a.ldv, t_beg * NK, sm.kl, a.dv);
+    }
   }
   Frag<NP> qf[KS], gf[KS];
   float delta = 0.f, lse2 = INFINITY;
@@ -102,6 +119,7 @@ __global__ __launch_bounds__(256) void gqa_dq_kernel(GqaArgs a) {
     bias_r = bias[a.M] * kLog2e;
   }
 
+  GqaLane<D> ln;
   constexpr bool FIX = NP == 1;  // R and the sums of p k
   gq_f32x16 acc[OB], pk[FIX ? OB : 1];
   float rest = 0.f;
@@ -113,31 +131,42 @@ __global__ __launch_bounds__(256) void gqa_dq_kernel(GqaArgs a) {
 
   for (int t = t_beg; t < t_end; ++t) {
     uint16_t* buf = lds + (NBUF == 2 ? (t & 1) * S::BUF : 0);
-    if (NBUF == 1 && t != t_beg) __syncthreads();
-    kt.stash(buf);
-    vt.stash(buf + NP * PL);
-    if (t + 1 < t_end) {
-      kt.fetch(kbase, a.ldk, (t + 1) * NK, sm.kl, a.dk);
-      vt.fetch(vbase, a.ldv, (t + 1) * NK, sm.kl, a.dv);
+    if constexpr (DMA) {
+      gq_dma_wait();
+      __syncthreads();
+      if (t + 1 < t_end) {
+        uint16_t* next = lds + ((t + 1) & 1) * S::BUF;
+        kt.issue(kbase, a.ldk, (t + 1) * NK, sm.kl, next);
+        vt.issue(vbase, a.ldv, (t + 1) * NK, sm.kl, next + PL);
+      }
+    } else {
+      if (NBUF == 1 && t != t_beg) __syncthreads();
+      kt.stash(buf);
+      vt.stash(buf + NP * PL);
+      if (t + 1 < t_end) {
+        kt.fetch(kbase, a.ldk, (t + 1) * NK, sm.kl, a.dk);
+        vt.fetch(vbase, a.ldv, (t + 1) * NK, sm.kl, a.dv);
+      }
+      __syncthreads();
     }
-    __syncthreads();
     const uint16_t *Kt = buf, *Vt = buf + NP * PL;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const int k0 = t * NK + 32 * kb;
       if (k0 >= lim_hi) continue;
+      ln.renew();
       gq_f32x16 s = gq_zero(), dp = gq_zero();
       {
         gq_f32x16 lo = gq_zero(), lo2 = gq_zero();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          const Frag<NP> kf = gq_frag_row<NP, D, PL>(Kt, kb * 32 + l32, 2 * ks + h);
+          const Frag<NP> kf = gq_frag_row<NP, D, PL>(Kt, ln, kb * 32, ks);
           if constexpr (NP == 3) lo = gq_mfma_small(kf, qf[ks], lo);
           s = gq_mfma(kf.p[0], qf[ks].p[0], s);
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          const Frag<NP> vf = gq_frag_row<NP, D, PL>(Vt, kb * 32 + l32, 2 * ks + h);
+          const Frag<NP> vf = gq_frag_row<NP, D, PL>(Vt, ln, kb * 32, ks);
           if constexpr (NP == 3) lo2 = gq_mfma_small(vf, gf[ks], lo2);
           dp = gq_mfma(vf.p[0], gf[ks].p[0], dp);
         }
@@ -190,7 +219,7 @@ __global__ __launch_bounds__(256) void gqa_dq_kernel(GqaArgs a) {
         if constexpr (NP == 1) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const gq_bf16x8 f = gq_frag_tr<1, D, PL>(Kt, 32 * kb + 16 * u, 32 * i, lane).p[0];
+            const gq_bf16x8 f = gq_frag_tr<1, D, PL>(Kt, ln, 32 * kb + 16 * u, i).p[0];
             acc[i] = gq_mfma(f, df[u].p[0], acc[i]);
             pk[i] = gq_mfma(f, pf[u].p[0], pk[i]);
           }
@@ -199,7 +228,7 @@ __global__ __launch_bounds__(256) void gqa_dq_kernel(GqaArgs a) {
           Frag<NP> kf[2];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            kf[u] = gq_frag_tr<NP, D, PL>(Kt, 32 * kb + 16 * u, 32 * i, lane);
+            kf[u] = gq_frag_tr<NP, D, PL>(Kt, ln, 32 * kb + 16 * u, i);
             x = gq_mfma_small(kf[u], df[u], x);
           }
 #pragma unroll
@@ -274,28 +303,64 @@ __global__ __launch_bounds__(256) void gqa_dq_join_kernel(GqaArgs a) {
 }
 
 // Distances that an LDS array holds beyond -M .. M on each side: a block that is not wholly M or more away reaches at
-// most 62 further.
+// most 62 further (and lane 63's place, which gets zeros, is one more).
 constexpr int kSlack = 64;
+
+// Where the scores of a query that has none start from: far enough below any others at every scale within 1e-30 .. 1e30.
+constexpr float kUnseen = -3e38f;
+
+// The sums of an accumulator's diagonals: lane i gets the sum of the values whose column less row is i - 31 (lane 63:
+// zero). Rows 8 j + 0..3 are the registers 4 j .. 4 j + 3 of the lower half, 8 j + 4..7 of the upper. Each of four chains
+// takes its eight rows, one after the other, into a row moved up by a lane a step, in 64 lanes of which the first 32 meet
+// values; the four are then brought together 8 lanes apart.
+__device__ __forceinline__ float diagonals(const float (&v)[16]) {
+  float chain[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t lo[4], hi[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[4 * j + i]), 0u, false, false);
+      lo[i] = x[0];  // the lower half's value and zeros
+      hi[i] = x[1];  // the upper half's, moved down, and zeros
+    }
+    float c = __uint_as_float(lo[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i)  // wave_shr:1, zero into lane 0
+      c = __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(c), 0x138, 0xf, 0xf, true)) +
+          __uint_as_float(i < 4 ? lo[i] : hi[i - 4]);
+    chain[j] = c;  // lane l + 7 - (row - 8 j); nothing from lane 39 on
+  }
+  const int lane = threadIdx.x & 63;
+  float x = chain[3];
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    x += __uint_as_float(__builtin_amdgcn_ds_bpermute(4 * ((lane - 8 * (3 - j)) & 63), __float_as_uint(chain[j])));
+  return x;
+}
 
 template <typename T, int D, int NQ, int NBUF>
 struct DkvShape {
   static constexpr int NP = kPlanes<T>, KEYS = 128, BUF = 2 * NP * NQ * D;
-  static constexpr size_t tile_bytes = (size_t)NBUF * BUF * 2, stat_bytes = (size_t)NBUF * 2 * NQ * 4;
+  static constexpr size_t tile_bytes = (size_t)NBUF * BUF * 2;
   static size_t lds(bool dbias, int M) {
-    return tile_bytes + stat_bytes + (dbias ? (size_t)8 * (2 * M + 1 + 2 * kSlack) * 4 + 8 * 4 : 0);
+    return tile_bytes + (dbias ? (size_t)4 * (2 * M + 1 + 2 * kSlack) * 4 + 8 * 4 : 0);
   }
 };
 
 // BIAS: 0 none, 1 added, 2 added and its gradient wanted.
-template <typename T, int D, int NQ, int NBUF, int BIAS>
-__global__ __launch_bounds__(256) void gqa_dkv_kernel(GqaArgs a) {
+template <typename T, int D, int NQ, int NBUF, int BIAS, bool DMA>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T, D, DMA>))) void gqa_dkv_kernel(GqaArgs a) {
   using S = DkvShape<T, D, NQ, NBUF>;
   constexpr int NP = S::NP, KS = D / 16, OB = D / 32, QB = NQ / 32, PL = NQ * D;
   extern __shared__ __align__(16) uint16_t lds[];
-  float* const stats = reinterpret_cast<float*>(reinterpret_cast<char*>(lds) + S::tile_bytes);  // [NBUF][lse2, D][NQ]
-  float* const far = stats + S::stat_bytes / 4;  // [4 waves][left, right]
-  float* const dist = far + 8;                   // [8 half waves][W]
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, wv = threadIdx.x >> 6;
+  float* const far = reinterpret_cast<float*>(reinterpret_cast<char*>(lds) + S::tile_bytes);  // [4 waves][left, right]
+  float* const dist = far + 8;                                                                  // [4 waves][W]
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, wv = gq_wave();
+  // Scores and dP start from -lse and -D in their accumulators; for the bias gradient, whose sums run over whole columns
+  // of them, both are added afterwards as the dQ kernel does, so that the two kernels' dS agree: accumulators round
+  // towards minus infinity, at the size of what they hold.
+  constexpr bool INIT = BIAS != 2;
   const GqaItem it = gq_item(a, false);
   const GqaSample sm = gq_sample(a, it.b);
   const int key0 = it.tile * S::KEYS, k0 = key0 + wv * 32, key = k0 + l32;
@@ -325,31 +390,39 @@ __global__ __launch_bounds__(256) void gqa_dkv_kernel(GqaArgs a) {
       vf[s] = gq_frag(g);
     }
   }
+  GqaLane<D> ln;
   gq_f32x16 dk[OB], dv[OB];
 #pragma unroll
   for (int i = 0; i < OB; ++i) dk[i] = dv[i] = gq_zero();
 
-  GqaTile<T, D, NQ> qt, gt;
-  float lse_r = 0.f, delta_r = 0.f;
+  std::conditional_t<DMA, GqaDma<D, NQ>, GqaTile<T, D, NQ>> qt, gt;
+  if constexpr (DMA) {
+    qt.init(a.ldq);
+    gt.init(a.lddo);
+  }
+  // of the next tile's query l32 in each block of 32: what its scores and dP start from
+  float s0_next[QB], dp0_next[QB];
   const T* qb0 = static_cast<const T*>(a.q) + (long long)it.b * a.Sq * a.ldq;
   const T* gb0 = static_cast<const T*>(a.dout) + (long long)it.b * a.Sq * a.lddo;
-  auto fetch = [&](int g, int t) {
+  auto fetch = [&](int g, int t, uint16_t* to) {
     const int head = it.kvh * a.G + g;
-    qt.fetch(qb0 + (long long)head * a.dk, a.ldq, t * NQ, sm.ql, a.dk);
-    gt.fetch(gb0 + (long long)head * a.dv, a.lddo, t * NQ, sm.ql, a.dv);
-    if (threadIdx.x < NQ) {
-      const int q = t * NQ + threadIdx.x;
-      lse_r = INFINITY;
-      delta_r = 0.f;
-      if (q < sm.ql) {
-        const long long at = ((long long)it.b * a.H + head) * a.Sq + q;
-        const float x = a.lse[at];
-        lse_r = x == -INFINITY ? INFINITY : x * kLog2e;
-        delta_r = a.delta[at];
-      }
+    if constexpr (DMA) {
+      qt.issue(qb0 + (long long)head * a.dk, a.ldq, t * NQ, sm.ql, to);
+      gt.issue(gb0 + (long long)head * a.dv, a.lddo, t * NQ, sm.ql, to + PL);
+    } else {
+      qt.fetch(qb0 + (long long)head * a.dk, a.ldq, t * NQ, sm.ql, a.dk);
+      gt.fetch(gb0 + (long long)head * a.dv, a.lddo, t * NQ, sm.ql, a.dv);
+    }
+    const long long at = ((long long)it.b * a.H + head) * a.Sq;
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      const int q = t * NQ + 32 * qb + l32;
+      s0_next[qb] = q < sm.ql ? a.lse[at + q] : -INFINITY;
+      dp0_next[qb] = q < sm.ql ? -a.delta[at + q] : 0.f;
     }
   };
-  if (q_beg < q_end) fetch(g_beg, q_beg);
+  if (q_beg < q_end) fetch(g_beg, q_beg, lds);
+  const float inv_scale = 1.f / a.scale;
   int n = 0;  // tiles done
   for (int g = g_beg; g < g_end; ++g) {
     const int head = it.kvh * a.G + g;
@@ -360,41 +433,51 @@ __global__ __launch_bounds__(256) void gqa_dkv_kernel(GqaArgs a) {
       bias_l = bias[-a.M] * kLog2e;
       bias_r = bias[a.M] * kLog2e;
     }
-    float* mine = dist + (wv * 2 + h) * W + a.M + kSlack;
+    float* mine = dist + wv * W + a.M + kSlack;
     if (BIAS == 2) {
-      for (int i = threadIdx.x; i < 8 * W; i += 256) dist[i] = 0.f;
+      for (int i = threadIdx.x; i < 4 * W; i += 256) dist[i] = 0.f;
       __syncthreads();
     }
     for (int t = q_beg; t < q_end; ++t, ++n) {
       uint16_t* buf = lds + (NBUF == 2 ? (n & 1) * S::BUF : 0);
-      float* st = stats + (NBUF == 2 ? (n & 1) * 2 * NQ : 0);
       if (NBUF == 1 && n) __syncthreads();
-      qt.stash(buf);
-      gt.stash(buf + NP * PL);
-      if (threadIdx.x < NQ) {
-        st[threadIdx.x] = lse_r;
-        st[NQ + threadIdx.x] = delta_r;
+      if constexpr (!DMA) {
+        qt.stash(buf);
+        gt.stash(buf + NP * PL);
       }
-      if (t + 1 < q_end) fetch(g, t + 1);
-      else if (g + 1 < g_end) fetch(g + 1, q_beg);
-      __syncthreads();
+      float s0[QB], dp0[QB];
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        // -lse in the scores' own units; a query past the sample's, or one that saw no key: every p is 0
+        s0[qb] = s0_next[qb] == -INFINITY ? kUnseen : -s0_next[qb] * inv_scale;
+        dp0[qb] = dp0_next[qb];
+      }
+      uint16_t* next = lds + (NBUF == 2 ? ((n + 1) & 1) * S::BUF : 0);
+      if constexpr (DMA) {
+        gq_dma_wait();
+        __syncthreads();
+      }
+      if (t + 1 < q_end) fetch(g, t + 1, next);
+      else if (g + 1 < g_end) fetch(g + 1, q_beg, next);
+      if constexpr (!DMA) __syncthreads();
       const uint16_t *Qt = buf, *Gt = buf + NP * PL;
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         const int q0 = t * NQ + 32 * qb;
         if (q0 >= sm.ql || k0 >= sm.kl || (a.causal && k0 > q0 + 31 + sm.off)) continue;
-        gq_f32x16 s = gq_zero(), dp = gq_zero();
+        ln.renew();
+        gq_f32x16 s = INIT ? gq_rows(s0[qb], h) : gq_zero(), dp = INIT ? gq_rows(dp0[qb], h) : gq_zero();
         {
           gq_f32x16 lo = gq_zero(), lo2 = gq_zero();
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
-            const Frag<NP> f = gq_frag_row<NP, D, PL>(Qt, qb * 32 + l32, 2 * ks + h);
+            const Frag<NP> f = gq_frag_row<NP, D, PL>(Qt, ln, qb * 32, ks);
             if constexpr (NP == 3) lo = gq_mfma_small(f, kf[ks], lo);
             s = gq_mfma(f.p[0], kf[ks].p[0], s);
           }
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
-            const Frag<NP> f = gq_frag_row<NP, D, PL>(Gt, qb * 32 + l32, 2 * ks + h);
+            const Frag<NP> f = gq_frag_row<NP, D, PL>(Gt, ln, qb * 32, ks);
             if constexpr (NP == 3) lo2 = gq_mfma_small(f, vf[ks], lo2);
             dp = gq_mfma(f.p[0], vf[ks].p[0], dp);
           }
@@ -425,7 +508,7 @@ __global__ __launch_bounds__(256) void gqa_dkv_kernel(GqaArgs a) {
           }
         }
         if (k0 + 31 >= sm.kl || (a.causal && k0 + 31 > q0 + sm.off)) {
-          // queries past the sample's are no matter here: their lse2 is infinite, their rows zero
+          // queries past the sample's are no matter here: their scores start from kUnseen
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (key >= sm.kl || (a.causal && key > q0 + gq_row(r, h) + sm.off)) {
@@ -434,23 +517,24 @@ __global__ __launch_bounds__(256) void gqa_dkv_kernel(GqaArgs a) {
             }
         }
         float p[16], ds[16];
+        if constexpr (INIT) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float4 ls = *reinterpret_cast<const float4*>(st + 32 * qb + 8 * j + 4 * h);
-          const float4 de = *reinterpret_cast<const float4*>(st + NQ + 32 * qb + 8 * j + 4 * h);
-          const float l4[4] = {ls.x, ls.y, ls.z, ls.w}, d4[4] = {de.x, de.y, de.z, de.w};
+          for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, add));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            p[4 * j + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], mul, add - l4[i]));
-            ds[4 * j + i] = p[4 * j + i] * (dp[4 * j + i] - d4[i]);
-          }
+          for (int r = 0; r < 16; ++r) ds[r] = p[r] * dp[r];
+        } else {
+          const gq_f32x16 ls = gq_rows(s0[qb] == kUnseen ? -1e30f : s0[qb] * a.c, h);  // finite pieces
+#pragma unroll
+          for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, add + ls[r]));
+          const gq_f32x16 de = gq_rows(dp0[qb], h);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) ds[r] = p[r] * (dp[r] + de[r]);
         }
         if (BIAS == 2) {
           if (side == 0) {
-            float* at = mine + key - q0 - sm.off;
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              __builtin_amdgcn_ds_atomic_fadd_f32((__attribute__((address_space(3))) float*)(at - gq_row(r, h)), ds[r]);
+            const float x = diagonals(ds);
+            // lane 63's is zero, and its place within the slack
+            mine[k0 - q0 - sm.off - 31 + lane] += x;
           } else {
             float x = 0.f;
 #pragma unroll
@@ -466,8 +550,8 @@ __global__ __launch_bounds__(256) void gqa_dkv_kernel(GqaArgs a) {
           if constexpr (NP == 1) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              dv[i] = gq_mfma(gq_frag_tr<1, D, PL>(Gt, 32 * qb + 16 * u, 32 * i, lane).p[0], pf[u].p[0], dv[i]);
-              dk[i] = gq_mfma(gq_frag_tr<1, D, PL>(Qt, 32 * qb + 16 * u, 32 * i, lane).p[0], df[u].p[0], dk[i]);
+              dv[i] = gq_mfma(gq_frag_tr<1, D, PL>(Gt, ln, 32 * qb + 16 * u, i).p[0], pf[u].p[0], dv[i]);
+              dk[i] = gq_mfma(gq_frag_tr<1, D, PL>(Qt, ln, 32 * qb + 16 * u, i).p[0], df[u].p[0], dk[i]);
             }
           } else {
 #pragma unroll
@@ -476,7 +560,7 @@ __global__ __launch_bounds__(256) void gqa_dkv_kernel(GqaArgs a) {
               Frag<NP> f[2];
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
-                f[u] = gq_frag_tr<NP, D, PL>(which ? Qt : Gt, 32 * qb + 16 * u, 32 * i, lane);
+                f[u] = gq_frag_tr<NP, D, PL>(which ? Qt : Gt, ln, 32 * qb + 16 * u, i);
                 x = gq_mfma_small(f[u], which ? df[u] : pf[u], x);
               }
 #pragma unroll
@@ -499,16 +583,13 @@ __global__ __launch_bounds__(256) void gqa_dkv_kernel(GqaArgs a) {
       const int n_out = 2 * a.M + 1;
       float* part = a.dbias_part +
                     ((((long long)it.b * a.H + head) * a.tiles + it.tile) * a.splits_q + part_q) * n_out;
-      for (int i = threadIdx.x; i < n_out; i += 256) {
-        // the ends take every distance beyond them
-        const int lo = i == 0 ? 0 : i + kSlack, hi = i == n_out - 1 ? W : i + kSlack + 1;
-        float x = 0.f;
-        for (int e = lo; e < hi; ++e)
-#pragma unroll
-          for (int w = 0; w < 8; ++w) x += dist[w * W + e];
-        if (i == 0) x += (far[0] + far[2]) + (far[4] + far[6]);
-        if (i == n_out - 1) x += (far[1] + far[3]) + (far[5] + far[7]);
-        part[i] = x;
+      auto fold = [&](int e) { return (dist[e] + dist[W + e]) + (dist[2 * W + e] + dist[3 * W + e]); };
+      for (int i = 1 + threadIdx.x; i < n_out - 1; i += 256) part[i] = fold(i + kSlack);
+      // the ends take every distance beyond them: a wave each
+      if (wv < 2) {
+        const int at = wv == 0 ? 0 : W - kSlack - 1;
+        const float x = wave_sum(fold(at + lane) + (lane == 0 ? fold(at + kSlack) : 0.f));
+        if (lane == 0) part[wv == 0 ? 0 : n_out - 1] = x + ((far[wv] + far[2 + wv]) + (far[4 + wv] + far[6 + wv]));
       }
       __syncthreads();  // before the next head's arrays are cleared
     }
@@ -565,16 +646,19 @@ struct BwdShape {
   size_t dq_lds;
   size_t (*dkv_lds)(bool, int);
 };
-template <typename T, int D, int NK, int NBK, int NQ, int NBQ>
+template <typename T, int D, int NK, int NBK, int NQ, int NBQ, bool DMA = false>
 BwdShape bwd_shape() {
-  return {{(const void*)gqa_dq_kernel<T, D, NK, NBK, 0>, (const void*)gqa_dq_kernel<T, D, NK, NBK, 1>},
-          {(const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 0>, (const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 1>,
-           (const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 2>},
+  return {{(const void*)gqa_dq_kernel<T, D, NK, NBK, false, DMA>, (const void*)gqa_dq_kernel<T, D, NK, NBK, true, DMA>},
+          {(const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 0, DMA>, (const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 1, DMA>,
+           (const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 2, DMA>},
           NK, NQ, DqShape<T, D, NK, NBK>::lds, DkvShape<T, D, NQ, NBQ>::lds};
 }
 template <typename T>
-BwdShape pick_bwd(int d) {
+BwdShape pick_bwd(int d, bool dma) {
   if constexpr (sizeof(T) == 2) {
+    if (dma && d == 32) return bwd_shape<T, 32, 64, 2, 64, 2, true>();
+    if (dma && d == 64) return bwd_shape<T, 64, 64, 2, 64, 2, true>();
+    if (dma && d == 128) return bwd_shape<T, 128, 32, 2, 32, 2, true>();
     if (d <= 32) return bwd_shape<T, 32, 64, 2, 32, 2>();
     if (d <= 64) return bwd_shape<T, 64, 64, 2, 32, 2>();
     return bwd_shape<T, 128, 32, 2, 32, 2>();
@@ -592,7 +676,7 @@ int launch(const void* fn, size_t blocks, size_t lds, GqaArgs* a, hipStream_t s,
   return hip_status(hipLaunchKernel(fn, dim3((unsigned)blocks), dim3(256), args, lds, s), name);
 }
 
-constexpr int kDbiasMaxDistance = 512;  // eight arrays of 2 M + 129 floats beside the tiles in a workgroup's LDS
+constexpr int kDbiasMaxDistance = 512;  // four arrays of 2 M + 129 floats beside the tiles in a workgroup's LDS
 constexpr long long kFill = 512;        // workgroups that fill the device: two a compute unit
 
 template <typename T>
@@ -625,7 +709,9 @@ int bwd(const char* fn, const talos_gqa_cfg* cfg, const int32_t* q_lens, const i
   a.lddk = ld_dk;
   a.dval = dv;
   a.lddv = ld_dv;
-  const BwdShape shape = pick_bwd<T>(std::max(a.dk, a.dv));
+  const bool dma = a.dk == a.dv && gq_dma_fits(q, ld_q) && gq_dma_fits(k, ld_k) && gq_dma_fits(v, ld_v) &&
+                   gq_dma_fits(dout, ld_do);
+  const BwdShape shape = pick_bwd<T>(std::max(a.dk, a.dv), dma);
 
   // parts of the key loop (dQ), of the heads and then of the query loop (dK, dV) where there is too little to do
   const long long pairs = (long long)a.B * a.KV;
@@ -634,8 +720,10 @@ int bwd(const char* fn, const talos_gqa_cfg* cfg, const int32_t* q_lens, const i
   long long sp_k = q_base ? std::min((kFill + q_base - 1) / q_base, ((long long)a.Sk + 255) / 256) : 1;
   sp_k = std::max(1ll, sp_k);
   long long sp_h = 1, sp_q = 1;
-  if (k_base && k_base < kFill) {
-    const long long want = (kFill + k_base - 1) / k_base;
+  // a causal key tile's share of the work, and a sample's, differ: twice the parts even them out
+  const long long fill = a.causal || q_lens || k_lens ? 2 * kFill : kFill;
+  if (k_base && k_base < fill) {
+    const long long want = (fill + k_base - 1) / k_base;
     for (long long d = 1; d <= a.G; ++d)  // the least divisor of the group that is enough, or the whole group
       if (a.G % d == 0 && (d >= want || d == a.G)) {
         sp_h = d;

@@ -15,6 +15,7 @@
 // keys of a tile four times as long, and their results are joined in LDS. Few workgroups: the keys are cut into
 // parts, each with its own maximum and sum, joined by a second kernel.
 #include <algorithm>
+#include <type_traits>
 
 #include "gqa.hpp"
 
@@ -30,13 +31,20 @@ struct FwdShape {
   static constexpr size_t lds = std::max((size_t)NBUF * BUF * 2, join_bytes);
 };
 
-// BIAS: 0 none, 1 by distance.
-template <typename T, int D, int NK, int KW, int NBUF, int BIAS>
-__global__ __launch_bounds__(256) void gqa_fwd_kernel(GqaArgs a) {
+// Two waves a SIMD (a wave's softmax beside another's products): 256 registers a lane, which the bf16 kernels and
+// the fp32 ones to 64 columns fit; with no such bound the compiler keeps accumulators in the other register file and
+// moves them for every tile (4 x 4096 tokens, d 128: 557 us).
+template <typename T, int D>
+constexpr int kFwdWaves = sizeof(T) == 4 && D == 128 ? 1 : 2;
+
+// BIAS: by distance. DMA: bf16 tiles go from memory to LDS directly.
+template <typename T, int D, int NK, int KW, int NBUF, bool BIAS, bool DMA>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T, D>))) void gqa_fwd_kernel(GqaArgs a) {
+  static_assert(!DMA || (sizeof(T) == 2 && (NBUF == 2 || KW > 1)), "direct tiles are bf16, shared ones land in the other buffer");
   using S = FwdShape<T, D, NK, KW, NBUF>;
   constexpr int NP = S::NP, TK = S::TK, KS = D / 16, OB = D / 32, KB = NK / 32, PL = TK * D;
   extern __shared__ __align__(16) uint16_t lds[];
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, wv = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, wv = gq_wave();
   const int wr = wv / KW, kw = wv % KW;
   const GqaItem it = gq_item(a, true);
   const GqaSample sm = gq_sample(a, it.b);
@@ -58,10 +66,27 @@ __global__ __launch_bounds__(256) void gqa_fwd_kernel(GqaArgs a) {
 
   const T* kbase = static_cast<const T*>(a.k) + (long long)it.b * a.Sk * a.ldk + (long long)it.kvh * a.dk;
   const T* vbase = static_cast<const T*>(a.v) + (long long)it.b * a.Sk * a.ldv + (long long)it.kvh * a.dv;
-  GqaTile<T, D, TK> kt, vt;
-  if (t_beg < t_end) {
-    kt.fetch(kbase, a.ldk, t_beg * TK, sm.kl, a.dk);
-    vt.fetch(vbase, a.ldv, t_beg * TK, sm.kl, a.dv);
+  // few rows and direct tiles: each wave streams the tiles of its own keys and meets the others only at the end
+  constexpr bool ALONE = DMA && KW > 1;
+  std::conditional_t<DMA, GqaDma<D, ALONE ? NK : TK, ALONE ? 1 : 4>, GqaTile<T, D, TK>> kt, vt;
+  if constexpr (DMA) {
+    kt.init(a.ldk);
+    vt.init(a.ldv);
+  }
+  if constexpr (ALONE) {
+    if (t_beg < t_end && t_beg * TK + kw * NK < lim_hi) {
+      kt.issue(kbase, a.ldk, t_beg * TK + kw * NK, sm.kl, lds + kw * NK * D);
+      vt.issue(vbase, a.ldv, t_beg * TK + kw * NK, sm.kl, lds + PL + kw * NK * D);
+    }
+  } else if (t_beg < t_end) {
+    if constexpr (DMA) {
+      uint16_t* buf = lds + (t_beg & 1) * S::BUF;
+      kt.issue(kbase, a.ldk, t_beg * TK, sm.kl, buf);
+      vt.issue(vbase, a.ldv, t_beg * TK, sm.kl, buf + PL);
+    } else {
+      kt.fetch(kbase, a.ldk, t_beg * TK, sm.kl, a.dk);
+      vt.fetch(vbase, a.ldv, t_beg * TK, sm.kl, a.dv);
+    }
   }
   Frag<NP> qf[KS];
   {
@@ -84,6 +109,7 @@ __global__ __launch_bounds__(256) void gqa_fwd_kernel(GqaArgs a) {
     bias_r = bias[a.M] * kLog2e;
   }
 
+  GqaLane<D> ln;
   float m = -INFINITY, l = 0.f;
   gq_f32x16 acc[OB];
 #pragma unroll
@@ -91,24 +117,39 @@ __global__ __launch_bounds__(256) void gqa_fwd_kernel(GqaArgs a) {
 
   for (int t = t_beg; t < t_end; ++t) {
     uint16_t* buf = lds + (NBUF == 2 ? (t & 1) * S::BUF : 0);
-    if (NBUF == 1 && t != t_beg) __syncthreads();  // the last tile's readers are done
-    kt.stash(buf);
-    vt.stash(buf + NP * PL);
-    if (t + 1 < t_end) {
-      kt.fetch(kbase, a.ldk, (t + 1) * TK, sm.kl, a.dk);
-      vt.fetch(vbase, a.ldv, (t + 1) * TK, sm.kl, a.dv);
-    }
-    __syncthreads();
     const int k0 = t * TK + kw * NK;  // this wave's keys
+    const bool more = t + 1 < t_end && k0 + TK < lim_hi;
+    if constexpr (ALONE) {
+      // in flight, in order: K of this tile, V of this tile
+      if (k0 < lim_hi) gq_dma_wait<decltype(vt)::PER>();
+    } else if constexpr (DMA) {
+      gq_dma_wait();
+      __syncthreads();  // tile t is here, and the other buffer's readers are done
+      if (t + 1 < t_end) {
+        uint16_t* next = lds + ((t + 1) & 1) * S::BUF;
+        kt.issue(kbase, a.ldk, (t + 1) * TK, sm.kl, next);
+        vt.issue(vbase, a.ldv, (t + 1) * TK, sm.kl, next + PL);
+      }
+    } else {
+      if (NBUF == 1 && t != t_beg) __syncthreads();  // the last tile's readers are done
+      kt.stash(buf);
+      vt.stash(buf + NP * PL);
+      if (t + 1 < t_end) {
+        kt.fetch(kbase, a.ldk, (t + 1) * TK, sm.kl, a.dk);
+        vt.fetch(vbase, a.ldv, (t + 1) * TK, sm.kl, a.dv);
+      }
+      __syncthreads();
+    }
     if (k0 >= lim_hi) continue;
     const uint16_t *Kt = buf + kw * NK * D, *Vt = buf + NP * PL + kw * NK * D;
+    ln.renew();
     gq_f32x16 s[KB];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       gq_f32x16 hi = gq_zero(), lo = gq_zero();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const Frag<NP> kf = gq_frag_row<NP, D, PL>(Kt, kb * 32 + l32, 2 * ks + h);
+        const Frag<NP> kf = gq_frag_row<NP, D, PL>(Kt, ln, kb * 32, ks);
         if constexpr (NP == 3) lo = gq_mfma_small(kf, qf[ks], lo);
         hi = gq_mfma(kf.p[0], qf[ks].p[0], hi);
       }
@@ -118,6 +159,17 @@ __global__ __launch_bounds__(256) void gqa_fwd_kernel(GqaArgs a) {
       }
       s[kb] = hi;
     }
+    if constexpr (ALONE) {
+      gq_reads_done();
+      if (more) kt.issue(kbase, a.ldk, k0 + TK, sm.kl, lds + kw * NK * D);
+    }
+    // the first fragments of V: on their way from LDS beside the softmax
+    constexpr int PRE = NP == 1 && !ALONE ? (2 < OB ? 2 : OB) : 0;
+    Frag<NP> early[PRE ? PRE : 1][2 * KB];
+#pragma unroll
+    for (int i = 0; i < PRE; ++i)
+#pragma unroll
+      for (int u = 0; u < 2 * KB; ++u) early[i][u] = gq_frag_tr<NP, D, PL>(Vt, ln, 16 * u, i);
     // scores in units of log 2, bias and mask included, less nothing yet; their maximum
     float add = 0.f;  // what every score of the row still lacks
     bool raw = true;  // s still lacks the factor c too
@@ -177,19 +229,23 @@ __global__ __launch_bounds__(256) void gqa_fwd_kernel(GqaArgs a) {
       pf[2 * kb + 1] = gq_frag_acc<NP>(p + 8);
     }
     l += sum;
+    if constexpr (ALONE) {
+      if (more) gq_dma_wait<decltype(kt)::PER>();
+      else gq_dma_wait();
+    }
 #pragma unroll
     for (int i = 0; i < OB; ++i) {
       if constexpr (NP == 1) {
 #pragma unroll
         for (int u = 0; u < 2 * KB; ++u)
-          acc[i] = gq_mfma(gq_frag_tr<1, D, PL>(Vt, 16 * u, 32 * i, lane).p[0], pf[u].p[0], acc[i]);
+          acc[i] = gq_mfma(i < PRE ? early[i < PRE ? i : 0][u].p[0] : gq_frag_tr<1, D, PL>(Vt, ln, 16 * u, i).p[0], pf[u].p[0], acc[i]);
       } else {
         // the tile's product by itself, the small pairs first, then one fp32 addition
         gq_f32x16 x = gq_zero();
         Frag<NP> vf[2 * KB];
 #pragma unroll
         for (int u = 0; u < 2 * KB; ++u) {
-          vf[u] = gq_frag_tr<NP, D, PL>(Vt, 16 * u, 32 * i, lane);
+          vf[u] = gq_frag_tr<NP, D, PL>(Vt, ln, 16 * u, i);
           x = gq_mfma_small(vf[u], pf[u], x);
         }
 #pragma unroll
@@ -197,6 +253,10 @@ __global__ __launch_bounds__(256) void gqa_fwd_kernel(GqaArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] += x[r];
       }
+    }
+    if constexpr (ALONE) {
+      gq_reads_done();
+      if (more) vt.issue(vbase, a.ldv, k0 + TK, sm.kl, lds + PL + kw * NK * D);
     }
   }
   l = gq_sum_halves(l);
@@ -315,16 +375,20 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(int parts, size_t rows, i
   gq_store4(out + row * ld, c, cols, x);
 }
 
-template <typename T, int D, int NK, int KW, int NBUF>
+template <typename T, int D, int NK, int KW, int NBUF, bool DMA = false>
 int fwd_launch(GqaArgs a, hipStream_t s) {
   using S = FwdShape<T, D, NK, KW, NBUF>;
-  const void* fn = a.bias ? (const void*)gqa_fwd_kernel<T, D, NK, KW, NBUF, 1> : (const void*)gqa_fwd_kernel<T, D, NK, KW, NBUF, 0>;
+  const void* fn = a.bias ? (const void*)gqa_fwd_kernel<T, D, NK, KW, NBUF, true, DMA>
+                          : (const void*)gqa_fwd_kernel<T, D, NK, KW, NBUF, false, DMA>;
   if (S::lds > 65536) TALOS_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds));
   const long long rows = (long long)a.G * a.Sq;
   a.tiles = (int)((rows + S::ROWS - 1) / S::ROWS);
   const long long base = (long long)a.tiles * a.B * a.KV;
-  // Parts of the key loop where there are fewer workgroups than two a compute unit, each at least two tiles long.
-  long long splits = base >= 512 ? 1 : (512 + base - 1) / base;
+  // Parts of the key loop where there are fewer workgroups than two a compute unit, each at least two tiles long. One
+  // token's workgroups of samples of different lengths end at different times: twice as many there (64 samples of up to
+  // 4096 keys, 32 heads on 8, d 128: 130 us in one part, 122 with the join in two, 122 in four).
+  const long long fill = KW > 1 && a.klens ? 1024 : 512;
+  long long splits = base >= fill ? 1 : (fill + base - 1) / base;
   splits = std::max(1ll, std::min(splits, ((long long)a.Sk + 2 * S::TK - 1) / (2 * S::TK)));
   TALOS_REQUIRE(base * splits <= 0x7fffffffll, TALOS_ERR_UNSUPPORTED, "talos_gqa_fwd: %lld workgroups", base * splits);
   a.splits = (int)splits;
@@ -361,7 +425,11 @@ int fwd(const char* fn, const talos_gqa_cfg* cfg, const int32_t* q_lens, const i
   const int d = std::max(a.dk, a.dv);
   const bool few = (long long)a.G * a.Sq <= 32;  // one wave's rows: the waves split the keys
   if constexpr (sizeof(T) == 2) {
-    if (d <= 32) rc = few ? fwd_launch<T, 32, 32, 4, 1>(a, s) : fwd_launch<T, 32, 64, 1, 2>(a, s);
+    const bool dma = a.dk == d && a.dv == d && gq_dma_fits(k, ld_k) && gq_dma_fits(v, ld_v);
+    if (dma && d == 32) rc = few ? fwd_launch<T, 32, 32, 4, 1, true>(a, s) : fwd_launch<T, 32, 64, 1, 2, true>(a, s);
+    else if (dma && d == 64) rc = few ? fwd_launch<T, 64, 32, 4, 1, true>(a, s) : fwd_launch<T, 64, 64, 1, 2, true>(a, s);
+    else if (dma && d == 128) rc = few ? fwd_launch<T, 128, 32, 4, 1, true>(a, s) : fwd_launch<T, 128, 32, 1, 2, true>(a, s);
+    else if (d <= 32) rc = few ? fwd_launch<T, 32, 32, 4, 1>(a, s) : fwd_launch<T, 32, 64, 1, 2>(a, s);
     else if (d <= 64) rc = few ? fwd_launch<T, 64, 32, 4, 1>(a, s) : fwd_launch<T, 64, 64, 1, 2>(a, s);
     else rc = few ? fwd_launch<T, 128, 32, 4, 1>(a, s) : fwd_launch<T, 128, 64, 1, 2>(a, s);
   } else {
@@ -398,6 +466,8 @@ int gqa_check(const char* fn, const talos_gqa_cfg* cfg, const float* bias, const
                 c.qk_dim, c.v_dim);
   TALOS_REQUIRE(c.causal == 0 || c.causal == 1, TALOS_ERR_DTYPE, "%s: causal must be 0 or 1", fn);
   TALOS_REQUIRE(c.scale > 0.f && c.scale < INFINITY, TALOS_ERR_SHAPE, "%s: scale must be positive and finite", fn);
+  TALOS_REQUIRE(c.scale >= 1e-30f && c.scale <= 1e30f, TALOS_ERR_UNSUPPORTED, "%s: scale %g is not within 1e-30 .. 1e30",
+                fn, (double)c.scale);
   TALOS_REQUIRE(!bias || (c.max_distance > 0 && c.max_distance <= (1 << 20)), TALOS_ERR_SHAPE,
                 "%s: a bias needs 1 <= max_distance <= 2^20, not %d", fn, c.max_distance);
   // rows of a sample's group and keys are counted in 32 bits (with a tile's length of room), addresses in 64

@@ -22,87 +22,120 @@ namespace talos {
 
 namespace {
 
-// Sum over the L lanes of a row, all of them receiving it. L = 256: the workgroup, through red[4].
+// Threads of a workgroup whose rows take L lanes.
 template <int L>
-__device__ __forceinline__ float row_sum(float v, float* red) {
+constexpr int kLnThreads = L > 256 ? L : 256;
+
+// Sums of a and b over the L lanes of a row, all of them receiving them. L > 64: the workgroup, through red[2 L / 64].
+template <int L>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
   if constexpr (L <= 64) {
-    return lanes_sum<L>(v);
+    a = lanes_sum<L>(a);
+    b = lanes_sum<L>(b);
   } else {
-    v = lanes_sum<64>(v);
+    constexpr int W = L / 64;
+    a = lanes_sum<64>(a);
+    b = lanes_sum<64>(b);
     __syncthreads();  // an earlier sum's readers are done with red
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) {
+      red[threadIdx.x >> 6] = a;
+      red[W + (threadIdx.x >> 6)] = b;
+    }
     __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
+    a = b = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      a += red[i];
+      b += red[W + i];
+    }
   }
 }
+template <int L>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  float none = 0.f;
+  row_sum2<L>(v, none, red);
+  return v;
+}
 
+// w and b stay in registers over the rows that a workgroup walks (read with every row they are four times a bf16 row's own
+// bytes: 8192 x 4096 bf16 37.4 us, 23.7 held), and the next row is on its way while one is reduced and written.
 template <typename T, int L, int V>
-__global__ __launch_bounds__(256) void layernorm_fwd_kernel(int rows, int dim, float eps, const T* __restrict__ x,
-                                                            const float* __restrict__ w, const float* __restrict__ b,
-                                                            T* __restrict__ y, float* __restrict__ mean_out,
-                                                            float* __restrict__ rstd_out) {
-  constexpr int N = Piece<T>::N;
-  __shared__ float red[4];
-  const long long row = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
-  const int lane = threadIdx.x % L;
-  if (row >= rows) return;  // L = 256: the whole workgroup
-  const T* xr = x + (size_t)row * dim;
-  float v[V][N];
-  float s = 0.f;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    load_piece(xr, N * (lane + L * j), dim, v[j]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) s += v[j][i];
-  }
+__global__ __launch_bounds__(kLnThreads<L>) void layernorm_fwd_kernel(int rows, int dim, float eps, const T* x,
+                                                                      const float* __restrict__ w,
+                                                                      const float* __restrict__ b, T* y,
+                                                                      float* __restrict__ mean_out,
+                                                                      float* __restrict__ rstd_out) {
+  constexpr int N = Piece<T>::N, R = kLnThreads<L> / L;
+  __shared__ float red[L > 64 ? 2 * L / 64 : 1];
+  const int lane = threadIdx.x % L, sub = threadIdx.x / L;
   const float inv = 1.0f / (float)dim;
-  const float mean = row_sum<L>(s, red) * inv;
-  float q = 0.f;
+  float ww[V][N], bb[V][N];
 #pragma unroll
   for (int j = 0; j < V; ++j)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[j][i] -= mean;
-      q += N * (lane + L * j) + i < dim ? v[j][i] * v[j][i] : 0.f;
+    for (int p = 0; p < N; p += 4) {
+      float t[4] = {};
+      load_piece(w, N * (lane + L * j) + p, dim, t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ww[j][p + i] = t[i];
+      if (b) load_piece(b, N * (lane + L * j) + p, dim, t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bb[j][p + i] = b ? t[i] : 0.f;
     }
-  const float rstd = 1.0f / sqrtf(row_sum<L>(q, red) * inv + eps);
-  if (lane == 0) {
-    if (mean_out) mean_out[row] = mean;
-    if (rstd_out) rstd_out[row] = rstd;
-  }
-  T* yr = y + (size_t)row * dim;
+  typename Piece<T>::Raw next[V];
+  auto fetch = [&](long long row) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int c = N * (lane + L * j);
-    if (c >= dim) continue;
-    float ww[N], bb[N];
+    for (int j = 0; j < V; ++j)
+      next[j] = load_raw(x + (size_t)(row < rows ? row : 0) * dim, row < rows ? N * (lane + L * j) : dim, dim);
+  };
+  const long long step = (long long)gridDim.x * R;
+  fetch((long long)blockIdx.x * R + sub);
+  for (long long row0 = (long long)blockIdx.x * R; row0 < rows; row0 += step) {
+    const long long row = row0 + sub;
+    float v[V][N];
+    float s = 0.f, q = 0.f;
 #pragma unroll
-    for (int k = 0; k < N; k += 4) {
-      float t[4];
-      load_piece(w, c + k, dim, t);
+    for (int j = 0; j < V; ++j) {
+      Piece<T>::widen(next[j], v[j]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ww[k + i] = t[i];
-      if (b) {
-        load_piece(b, c + k, dim, t);
+      for (int i = 0; i < N; ++i) s += v[j][i];
+    }
+    if (row0 + step < rows) fetch(row + step);
+    const float mean = row_sum<L>(s, red) * inv;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bb[k + i] = t[i];
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        v[j][i] -= mean;
+        q += N * (lane + L * j) + i < dim ? v[j][i] * v[j][i] : 0.f;
       }
+    const float rstd = 1.0f / sqrtf(row_sum<L>(q, red) * inv + eps);
+    if (row >= rows) continue;  // L > 64: never
+    if (lane == 0) {
+      if (mean_out) mean_out[row] = mean;
+      if (rstd_out) rstd_out[row] = rstd;
     }
+    T* yr = y + (size_t)row * dim;
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[j][i] = v[j][i] * rstd * ww[i] + (b ? bb[i] : 0.f);
-    store_piece(yr, c, dim, v[j]);
+    for (int j = 0; j < V; ++j) {
+      const int c = N * (lane + L * j);
+      if (c >= dim) continue;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[j][i] = v[j][i] * rstd * ww[j][i] + bb[j][i];
+      store_piece(yr, c, dim, v[j]);
+    }
   }
 }
 
 // Rows of any width: a workgroup a row, the row read three times (the second and third from cache).
 template <typename T>
-__global__ __launch_bounds__(256) void layernorm_fwd_wide_kernel(int rows, int dim, float eps, const T* __restrict__ x,
+__global__ __launch_bounds__(256) void layernorm_fwd_wide_kernel(int rows, int dim, float eps, const T* x,
                                                                  const float* __restrict__ w,
-                                                                 const float* __restrict__ b, T* __restrict__ y,
+                                                                 const float* __restrict__ b, T* y,
                                                                  float* __restrict__ mean_out,
                                                                  float* __restrict__ rstd_out) {
   constexpr int N = Piece<T>::N;
-  __shared__ float red[4];
+  __shared__ float red[8];
   const int row = blockIdx.x;
   const T* xr = x + (size_t)row * dim;
   T* yr = y + (size_t)row * dim;
@@ -138,14 +171,14 @@ __global__ __launch_bounds__(256) void layernorm_fwd_wide_kernel(int rows, int d
 
 // part: [gridDim.x][2 * dim] fp32, this workgroup's sums of g * xh, then of g (null: neither is wanted).
 template <typename T, int L, int V>
-__global__ __launch_bounds__(256) void layernorm_bwd_kernel(int rows, int dim, const T* __restrict__ x,
+__global__ __launch_bounds__(kLnThreads<L>) void layernorm_bwd_kernel(int rows, int dim, const T* __restrict__ x,
                                                             const float* __restrict__ w,
                                                             const float* __restrict__ mean,
                                                             const float* __restrict__ rstd, const T* dy,
                                                             int accumulate, T* dx, float* __restrict__ part) {
-  constexpr int N = Piece<T>::N, R = 256 / L;  // rows a workgroup takes at once
-  __shared__ float red[8];
-  __shared__ float cols[L == 256 ? 1 : 4 * 64 * N];
+  constexpr int N = Piece<T>::N, R = kLnThreads<L> / L;  // rows a workgroup takes at once
+  __shared__ float red[L > 64 ? 2 * L / 64 : 1];
+  __shared__ float cols[L > 64 ? 1 : 4 * 64 * N];
   const int lane = threadIdx.x % L, sub = threadIdx.x / L;
   const float inv = 1.0f / (float)dim;
   float ww[V][N], sw[V][N], sb[V][N];
@@ -161,18 +194,34 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(int rows, int dim, c
 #pragma unroll
     for (int i = 0; i < N; ++i) sw[j][i] = sb[j][i] = 0.f;
   }
-  for (long long row0 = (long long)blockIdx.x * R; row0 < rows; row0 += gridDim.x * R) {
-    const long long row = row0 + sub;
-    const bool on = row < rows;  // L = 256: always
-    float xh[V][N], g[V][N];
-    const float m = on ? mean[row] : 0.f, r = on ? rstd[row] : 0.f;
-    float s = 0.f, q = 0.f;
+  // the next rows' pieces and statistics are on their way while a row is reduced and written
+  typename Piece<T>::Raw nx[V], ng[V];
+  float nm = 0.f, nr = 0.f;
+  auto fetch = [&](long long row) {
+    const bool on = row < rows;
+    nm = on ? mean[row] : 0.f;
+    nr = on ? rstd[row] : 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int c = on ? N * (lane + L * j) : dim;
-      load_piece(x + (size_t)(on ? row : 0) * dim, c, dim, xh[j]);
-      load_piece(dy + (size_t)(on ? row : 0) * dim, c, dim, g[j]);
+      nx[j] = load_raw(x + (size_t)(on ? row : 0) * dim, c, dim);
+      ng[j] = load_raw(dy + (size_t)(on ? row : 0) * dim, c, dim);
     }
+  };
+  const long long step = (long long)gridDim.x * R;
+  fetch((long long)blockIdx.x * R + sub);
+  for (long long row0 = (long long)blockIdx.x * R; row0 < rows; row0 += step) {
+    const long long row = row0 + sub;
+    const bool on = row < rows;  // L > 64: always
+    float xh[V][N], g[V][N];
+    const float m = nm, r = nr;
+    float s = 0.f, q = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      Piece<T>::widen(nx[j], xh[j]);
+      Piece<T>::widen(ng[j], g[j]);
+    }
+    if (row0 + step < rows) fetch(row + step);
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
@@ -184,21 +233,7 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(int rows, int dim, c
         s += g[j][i];
         q += g[j][i] * xh[j][i];
       }
-    if constexpr (L <= 64) {
-      s = lanes_sum<L>(s);
-      q = lanes_sum<L>(q);
-    } else {
-      s = lanes_sum<64>(s);
-      q = lanes_sum<64>(q);
-      __syncthreads();
-      if ((threadIdx.x & 63) == 0) {
-        red[threadIdx.x >> 6] = s;
-        red[4 + (threadIdx.x >> 6)] = q;
-      }
-      __syncthreads();
-      s = (red[0] + red[1]) + (red[2] + red[3]);
-      q = (red[4] + red[5]) + (red[6] + red[7]);
-    }
+    row_sum2<L>(s, q, red);
     s *= inv;
     q *= inv;
     if (on) {
@@ -222,7 +257,7 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(int rows, int dim, c
   }
   if (part == nullptr) return;
   float* p = part + (size_t)blockIdx.x * 2 * dim;
-  if constexpr (L == 256) {
+  if constexpr (L > 64) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       store_piece(p, N * (lane + L * j), dim, *reinterpret_cast<float(*)[4]>(sw[j]));
@@ -265,7 +300,7 @@ __global__ __launch_bounds__(256) void layernorm_bwd_wide_kernel(int rows, int d
                                                                  const float* __restrict__ rstd,
                                                                  const T* dy, int accumulate, T* dx) {
   constexpr int N = Piece<T>::N;
-  __shared__ float red[4];
+  __shared__ float red[8];
   const int row = blockIdx.x;
   const T *xr = x + (size_t)row * dim, *gr = dy + (size_t)row * dim;
   T* dr = dx + (size_t)row * dim;
@@ -321,21 +356,27 @@ __global__ __launch_bounds__(256) void layernorm_cols_wide_kernel(int rows, int 
         (red[wv][0][l] + red[wv][1][l]) + (red[wv][2][l] + red[wv][3][l]);
 }
 
-// dw, db = beta * (dw, db) + the sum of nparts fp32 partial rows, in f64 and in a fixed order: 64 columns a
-// workgroup, its 16 waves every 16th partial row.
+// dw, db = beta * (dw, db) + the sum of nparts fp32 partial rows, in f64 and in a fixed order: C columns a workgroup, its
+// 1024 / C groups of C lanes every 1024 / C-th partial row. C = 16 where 64 would leave most compute units idle (256
+// columns of 512 partial rows: 11.0 us with 64, 4.7 with 16).
+template <int C>
 __global__ __launch_bounds__(1024) void layernorm_parts_kernel(int dim, int nparts, const float* __restrict__ part,
                                                                float beta, float* dw, float* db) {
-  __shared__ double red[16][64];
-  const int l = threadIdx.x & 63, wv = threadIdx.x >> 6, c = blockIdx.x * 64 + l, n = 2 * dim;
+  constexpr int G = 1024 / C;
+  __shared__ double red[G][C + 1];
+  const int l = threadIdx.x % C, g = threadIdx.x / C, c = blockIdx.x * C + l, n = 2 * dim;
   double s = 0.0;
   if (c < n)
-    for (int p = wv; p < nparts; p += 16) s += (double)part[(size_t)p * n + c];
-  red[wv][l] = s;
+    for (int p = g; p < nparts; p += G) s += (double)part[(size_t)p * n + c];
+  red[g][l] = s;
   __syncthreads();
-  if (wv != 0 || c >= n) return;
-  s = 0.0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s += red[i][l];
+  for (int o = G / 2; o > 0; o >>= 1) {
+    if (g < o) red[g][l] += red[g + o][l];
+    __syncthreads();
+  }
+  if (g != 0 || c >= n) return;
+  s = red[0][l];
   float* o = c < dim ? (dw ? dw + c : nullptr) : (db ? db + (c - dim) : nullptr);
   if (o) *o = (float)(s + (beta != 0.f ? (double)*o : 0.0));
 }
@@ -346,13 +387,14 @@ constexpr int kLnBlocks = 512;
 constexpr int kLnWideParts = 64;
 constexpr int kLnMaxDim = 1 << 26;
 
-// f(L, V) with the lanes a row and the pieces a lane for `dim`; false beyond 8192 values.
+// f(L, V) with the lanes a row and the pieces a lane for `dim`: 16 values a lane at most, which the backward holds beside
+// another row's and two sums a column; false beyond 8192 values.
 template <typename T, typename F>
 bool pick_shape(int dim, F&& f) {
-  constexpr int N = Piece<T>::N;
+  constexpr int N = Piece<T>::N, U = N == 4 ? 2 : 1;
   const int pieces = (dim + N - 1) / N;
 #define TALOS_LN_SHAPE(L, V)                                               \
-  if (pieces <= L * V) {                                                   \
+  if (pieces <= L * (V)) {                                                 \
     f(std::integral_constant<int, L>(), std::integral_constant<int, V>()); \
     return true;                                                           \
   }
@@ -361,15 +403,10 @@ bool pick_shape(int dim, F&& f) {
   TALOS_LN_SHAPE(32, 1)
   TALOS_LN_SHAPE(64, 1)
   TALOS_LN_SHAPE(64, 2)
-  TALOS_LN_SHAPE(64, 4)
-  if constexpr (N == 4) {
-    TALOS_LN_SHAPE(64, 8)
-    TALOS_LN_SHAPE(256, 4)
-    TALOS_LN_SHAPE(256, 8)
-  } else {
-    TALOS_LN_SHAPE(256, 2)
-    TALOS_LN_SHAPE(256, 4)
-  }
+  if constexpr (N == 4) TALOS_LN_SHAPE(64, 4)
+  TALOS_LN_SHAPE(256, U)
+  TALOS_LN_SHAPE(256, 2 * U)
+  TALOS_LN_SHAPE(1024, U)
 #undef TALOS_LN_SHAPE
   return false;
 }
@@ -377,7 +414,7 @@ bool pick_shape(int dim, F&& f) {
 template <typename T>
 int bwd_blocks(int rows, int dim) {
   int per = 1;
-  const bool held = pick_shape<T>(dim, [&](auto L, auto) { per = 256 / decltype(L)::value; });
+  const bool held = pick_shape<T>(dim, [&](auto L, auto) { per = kLnThreads<decltype(L)::value> / decltype(L)::value; });
   if (!held) return std::min<int>(kLnWideParts, (int)ceil_div(rows, 4));
   return std::min<int>(kLnBlocks, (int)ceil_div(rows, per));
 }
@@ -393,8 +430,11 @@ int layernorm_fwd(const char* fn, int rows, int dim, float eps, const T* x, cons
   if (rows == 0) return entry_done(TALOS_OK, s);
   const bool held = pick_shape<T>(dim, [&](auto L, auto V) {
     constexpr int kL = decltype(L)::value, kV = decltype(V)::value;
-    hipLaunchKernelGGL((layernorm_fwd_kernel<T, kL, kV>), dim3(ceil_div(rows, 256 / kL)), dim3(256), 0, s, rows, dim,
-                       eps, x, w, b, y, mean, rstd);
+    // half of what the device holds at once: 1024 threads a compute unit
+    constexpr int kThreads = kLnThreads<kL>;
+    const unsigned blocks = std::min<unsigned>(ceil_div(rows, kThreads / kL), 128 * 2048 / kThreads);
+    hipLaunchKernelGGL((layernorm_fwd_kernel<T, kL, kV>), dim3(blocks), dim3(kThreads), 0, s, rows, dim, eps, x, w, b, y,
+                       mean, rstd);
   });
   if (!held)
     hipLaunchKernelGGL(layernorm_fwd_wide_kernel<T>, dim3(rows), dim3(256), 0, s, rows, dim, eps, x, w, b, y, mean,
@@ -419,8 +459,8 @@ int layernorm_bwd(const char* fn, int rows, int dim, const T* x, const float* w,
   float* part = static_cast<float*>(ws.ptr);
   if (rows > 0) {
     const bool held = pick_shape<T>(dim, [&](auto L, auto V) {
-      hipLaunchKernelGGL((layernorm_bwd_kernel<T, decltype(L)::value, decltype(V)::value>), dim3(nblk), dim3(256), 0,
-                         s, rows, dim, x, w, mean, rstd, dy, beta_dx != 0.f, dx, part);
+      constexpr int kL = decltype(L)::value;
+      hipLaunchKernelGGL((layernorm_bwd_kernel<T, kL, decltype(V)::value>), dim3(nblk), dim3(kLnThreads<kL>), 0, s, rows, dim, x, w, mean, rstd, dy, beta_dx != 0.f, dx, part);
     });
     if (!held) {
       // the column sums first: dx may be dy's own buffer
@@ -433,8 +473,12 @@ int layernorm_bwd(const char* fn, int rows, int dim, const T* x, const float* w,
     rc = launch_status("layernorm_bwd");
   }
   if (!rc && sums) {
-    hipLaunchKernelGGL(layernorm_parts_kernel, dim3(ceil_div((size_t)2 * dim, 64)), dim3(1024), 0, s, dim, nblk, part,
-                       beta_dw, dw, db);
+    if (dim <= 4096)
+      hipLaunchKernelGGL(layernorm_parts_kernel<16>, dim3(ceil_div((size_t)2 * dim, 16)), dim3(1024), 0, s, dim, nblk, part,
+                         beta_dw, dw, db);
+    else
+      hipLaunchKernelGGL(layernorm_parts_kernel<64>, dim3(ceil_div((size_t)2 * dim, 64)), dim3(1024), 0, s, dim, nblk, part,
+                         beta_dw, dw, db);
     rc = launch_status("layernorm_parts_kernel");
   }
   const int rel = ws.release();

@@ -77,6 +77,14 @@ __device__ __forceinline__ void load_piece(const T* row, int c, int dim, float (
     for (int i = 0; i < N; ++i) o[i] = c + i < dim ? to_f32(row[c + i]) : fill;
   }
 }
+// The piece as it is in memory, `fill` (a value of T that survives the round trip) past the row's end.
+template <typename T>
+__device__ __forceinline__ typename Piece<T>::Raw load_raw(const T* row, int c, int dim, float fill = 0.f) {
+  if (c + Piece<T>::N <= dim) return *reinterpret_cast<const typename Piece<T>::Raw*>(row + c);
+  float v[Piece<T>::N];
+  load_piece(row, c, dim, v, fill);
+  return Piece<T>::pack(v);
+}
 template <typename T>
 __device__ __forceinline__ void store_piece(T* row, int c, int dim, const float (&v)[Piece<T>::N]) {
   constexpr int N = Piece<T>::N;
