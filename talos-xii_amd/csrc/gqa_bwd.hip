@@ -39,7 +39,7 @@ struct DqShape {
 
 // waves a SIMD that the kernels are compiled for, as in the forward
 template <typename T, int D, bool DMA>
-constexpr int kBwdWaves = D == 128 ? (DMA ? 2 : 1) : sizeof(T) == 4 && D > 32 ? 1 : 2;
+constexpr int kBwdWaves = D == 128 && !DMA ? 1 : 2;
 
 // BIAS, DMA: as in the forward
 template <typename T, int D, int NK, int NBUF, bool BIAS, bool DMA>
@@ -677,7 +677,7 @@ int launch(const void* fn, size_t blocks, size_t lds, GqaArgs* a, hipStream_t s,
 }
 
 constexpr int kDbiasMaxDistance = 512;  // four arrays of 2 M + 129 floats beside the tiles in a workgroup's LDS
-constexpr long long kFill = 512;        // workgroups that fill the device: two a compute unit
+constexpr long long kFill = 512;  // workgroups that fill the device: two a compute unit
 
 template <typename T>
 int bwd(const char* fn, const talos_gqa_cfg* cfg, const int32_t* q_lens, const int32_t* k_lens, const float* bias,
@@ -717,13 +717,14 @@ int bwd(const char* fn, const talos_gqa_cfg* cfg, const int32_t* q_lens, const i
   const long long pairs = (long long)a.B * a.KV;
   const long long q_tiles = ((long long)a.G * a.Sq + 127) / 128, k_tiles = (a.Sk + 127) / 128;
   const long long q_base = pairs * q_tiles, k_base = pairs * k_tiles;
-  long long sp_k = q_base ? std::min((kFill + q_base - 1) / q_base, ((long long)a.Sk + 255) / 256) : 1;
+  const long long fill = kFill / (std::max(a.dk, a.dv) > 64 && !dma ? 2 : 1);  // where a wave has a SIMD to itself
+  long long sp_k = q_base ? std::min((fill + q_base - 1) / q_base, ((long long)a.Sk + 255) / 256) : 1;
   sp_k = std::max(1ll, sp_k);
   long long sp_h = 1, sp_q = 1;
   // a causal key tile's share of the work, and a sample's, differ: twice the parts even them out
-  const long long fill = a.causal || q_lens || k_lens ? 2 * kFill : kFill;
-  if (k_base && k_base < fill) {
-    const long long want = (fill + k_base - 1) / k_base;
+  const long long fill_k = a.causal || q_lens || k_lens ? 2 * fill : fill;
+  if (k_base && k_base < fill_k) {
+    const long long want = (fill_k + k_base - 1) / k_base;
     for (long long d = 1; d <= a.G; ++d)  // the least divisor of the group that is enough, or the whole group
       if (a.G % d == 0 && (d >= want || d == a.G)) {
         sp_h = d;

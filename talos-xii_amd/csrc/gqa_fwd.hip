@@ -335,19 +335,18 @@ __global__ __launch_bounds__(256) void gqa_fwd_join_kernel(GqaArgs a) {
   const int d = 4 * (threadIdx.x & 31), head = (int)(row % a.H);
   const long long token = row / a.H, at = (token / a.Sq * a.H + head) * a.Sq + token % a.Sq;
   float top = -INFINITY;
+#pragma unroll 4
   for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part1[s * rows + at]);
   float x[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+  if (top == -INFINITY) top = 0.f;  // no part saw a key
+#pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
-    const float ls = a.part1[s * rows + at];
-    if (ls == -INFINITY) continue;
-    const float w = __builtin_amdgcn_exp2f((ls - top) * kLog2e);
+    const float w = __builtin_amdgcn_exp2f((a.part1[s * rows + at] - top) * kLog2e);  // 0 of a part that saw none
+    float v[4] = {};
+    if (d < a.dv) load_piece(a.part0 + (s * rows + row) * a.dv, d, a.dv, v);
     sum += w;
-    if (d < a.dv) {
-      float v[4];
-      load_piece(a.part0 + (s * rows + row) * a.dv, d, a.dv, v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = fmaf(w, v[i], x[i]);
-    }
+    for (int i = 0; i < 4; ++i) x[i] = fmaf(w, v[i], x[i]);
   }
   if (d < a.dv) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -366,6 +365,7 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(int parts, size_t rows, i
   if (row >= rows) return;
   const int c = 4 * (int)(i % per);
   float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int p = 0; p < parts; ++p) {
     float v[4];
     load_piece(part + p * n + row * cols, c, cols, v);
@@ -384,12 +384,13 @@ int fwd_launch(GqaArgs a, hipStream_t s) {
   const long long rows = (long long)a.G * a.Sq;
   a.tiles = (int)((rows + S::ROWS - 1) / S::ROWS);
   const long long base = (long long)a.tiles * a.B * a.KV;
-  // Parts of the key loop where there are fewer workgroups than two a compute unit, each at least two tiles long. One
-  // token's workgroups of samples of different lengths end at different times: twice as many there (64 samples of up to
-  // 4096 keys, 32 heads on 8, d 128: 130 us in one part, 122 with the join in two, 122 in four).
-  const long long fill = KW > 1 && a.klens ? 1024 : 512;
+  // Parts of the key loop, of at least 128 keys, where there are fewer workgroups than the device holds: two a compute
+  // unit, or one of the kernels that need a SIMD's registers for a wave. One token's workgroups of samples of different
+  // lengths end at different times: twice as many there (64 samples of up to 4096 keys, 32 heads on 8, d 128: 130 us in
+  // one part, 122 with the join in two, 122 in four).
+  const long long fill = (KW > 1 && a.klens ? 1024 : 512) / (kFwdWaves<T, D> == 1 ? 2 : 1);
   long long splits = base >= fill ? 1 : (fill + base - 1) / base;
-  splits = std::max(1ll, std::min(splits, ((long long)a.Sk + 2 * S::TK - 1) / (2 * S::TK)));
+  splits = std::max(1ll, std::min(splits, ((long long)a.Sk + 127) / 128));
   TALOS_REQUIRE(base * splits <= 0x7fffffffll, TALOS_ERR_UNSUPPORTED, "talos_gqa_fwd: %lld workgroups", base * splits);
   a.splits = (int)splits;
   const size_t out_rows = (size_t)a.B * a.Sq * a.H;

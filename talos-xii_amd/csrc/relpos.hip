@@ -13,6 +13,8 @@
 //
 // So every bucket holds one run of distances, and the bias row of a head is [2 M + 1] values: d = -M .. M.
 // The gradient of a table entry is the sum of its run. Both are a few kilobytes: launch latency is all.
+#include <cmath>
+
 #include "common.hpp"
 
 namespace talos {
@@ -21,6 +23,7 @@ namespace {
 
 struct RelposArgs {
   int buckets, heads, max_distance, both;
+  double per_log;  // (S - E) / ln(M / E)
 };
 
 __device__ __forceinline__ int relpos_bucket(const RelposArgs& a, int d) {
@@ -28,8 +31,7 @@ __device__ __forceinline__ int relpos_bucket(const RelposArgs& a, int d) {
   const int n = a.both ? abs(d) : max(0, -d);
   int b = n;
   if (n >= few) {
-    const double step =
-        log((double)n / (double)few) / log((double)a.max_distance / (double)few) * (double)(side - few) + 1e-9;
+    const double step = log((double)n / (double)few) * a.per_log + 1e-9;
     b = n >= a.max_distance ? side - 1 : min(side - 1, few + (int)step);
   }
   return b + (a.both && d > 0 ? side : 0);
@@ -50,18 +52,29 @@ __global__ __launch_bounds__(256) void relpos_fwd_kernel(RelposArgs a, const flo
 constexpr int kRelposMaxBuckets = 4096, kRelposMaxDistance = 1 << 20;
 __global__ __launch_bounds__(256) void relpos_bwd_kernel(RelposArgs a, const float* __restrict__ dbias, float beta,
                                                          float* dtable) {
-  __shared__ int first[kRelposMaxBuckets], last[kRelposMaxBuckets];
+  __shared__ int first[kRelposMaxBuckets], last[kRelposMaxBuckets], of[256];
   const int n = 2 * a.max_distance + 1, h = blockIdx.x;
   for (int b = threadIdx.x; b < a.buckets; b += 256) {
     first[b] = 0;
     last[b] = -1;  // a bucket that no distance has
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const int b = relpos_bucket(a, i - a.max_distance);
-    if (i == 0 || relpos_bucket(a, i - 1 - a.max_distance) != b) first[b] = i;
-    if (i == n - 1 || relpos_bucket(a, i + 1 - a.max_distance) != b) last[b] = i;
+  // a run begins where the bucket is not the one before; 256 distances at a time, the last one's bucket handed on
+  int carried = -1;
+  for (int i0 = 0; i0 < n; i0 += 256) {
+    const int i = i0 + threadIdx.x;
+    const int b = i < n ? relpos_bucket(a, i - a.max_distance) : -1;
+    of[threadIdx.x] = b;
+    __syncthreads();
+    const int before = threadIdx.x ? of[threadIdx.x - 1] : carried;
+    if (b != before) {
+      if (b >= 0) first[b] = i;
+      if (before >= 0) last[before] = i - 1;
+    }
+    carried = of[255];
+    __syncthreads();
   }
+  if (threadIdx.x == 0 && carried >= 0) last[carried] = n - 1;
   __syncthreads();
   const int lane = threadIdx.x & 63;
   for (int b = threadIdx.x >> 6; b < a.buckets; b += 4) {
@@ -88,6 +101,11 @@ int check_relpos(const char* fn, int buckets, int heads, int max_distance, int b
   return TALOS_OK;
 }
 
+RelposArgs relpos_args(int buckets, int heads, int max_distance, int both) {
+  const int side = both ? buckets / 2 : buckets, few = side / 2;
+  return {buckets, heads, max_distance, both, (double)(side - few) / std::log((double)max_distance / (double)few)};
+}
+
 }  // namespace
 }  // namespace talos
 
@@ -102,7 +120,7 @@ int talos_relpos_bias_fwd_f32(int num_buckets, int heads, int max_distance, int 
   int rc = check_relpos(__func__, num_buckets, heads, max_distance, bidirectional);
   if (rc) return rc;
   TALOS_DEVICE();
-  const RelposArgs a{num_buckets, heads, max_distance, bidirectional};
+  const RelposArgs a = relpos_args(num_buckets, heads, max_distance, bidirectional);
   hipLaunchKernelGGL(relpos_fwd_kernel, dim3(ceil_div((size_t)2 * max_distance + 1, 256), heads), dim3(256), 0,
                      as_stream(stream), a, table, bias, buckets);
   return entry_done(launch_status("relpos_fwd_kernel"), as_stream(stream));
@@ -116,7 +134,7 @@ int talos_relpos_bias_bwd_f32(int num_buckets, int heads, int max_distance, int 
   if (rc) return rc;
   TALOS_REQUIRE(beta == 0.f || beta == 1.f, TALOS_ERR_UNSUPPORTED, "%s: beta must be 0 or 1", __func__);
   TALOS_DEVICE();
-  const RelposArgs a{num_buckets, heads, max_distance, bidirectional};
+  const RelposArgs a = relpos_args(num_buckets, heads, max_distance, bidirectional);
   hipLaunchKernelGGL(relpos_bwd_kernel, dim3(heads), dim3(256), 0, as_stream(stream), a, dbias, beta, dtable);
   return entry_done(launch_status("relpos_bwd_kernel"), as_stream(stream));
 }
