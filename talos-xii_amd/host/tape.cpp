@@ -386,6 +386,136 @@ Tensor RMSNorm::forward(const Tensor& x) const {
 std::vector<Tensor> RMSNorm::parameters() const { return {weight}; }
 
 // ---------------------------------------------------------------------------
+// Operators of policies over long histories
+// ---------------------------------------------------------------------------
+LayerNorm::LayerNorm(size_t dim, double e)
+    : weight(Tensor::from_vec(std::vector<double>(dim, 1.0), {dim})), bias(Tensor::zeros({dim})), eps(e) {}
+
+Tensor LayerNorm::forward(const Tensor& x) const {
+  const size_t dim = weight.numel();
+  require(!x.shape.empty() && x.shape.back() == dim, "LayerNorm dim mismatch");
+  const size_t rows = x.numel() / dim;
+  Tensor out = fresh(x.shape);
+  auto mean = std::make_shared<Storage>(rows), rstd = std::make_shared<Storage>(rows);
+  ok(talos_layernorm_fwd_f32((int)rows, (int)dim, (float)eps, x.data_->ptr, weight.data_->ptr, bias.data_->ptr,
+                             out.data_->ptr, mean->ptr, rstd->ptr, nullptr),
+     "layernorm_fwd");
+  return with_ctx(out, {x, weight, bias}, [mean, rstd, rows, dim](const Tensor& o, std::vector<Tensor>& p) {
+    ok(talos_layernorm_bwd_f32((int)rows, (int)dim, p[0].data_->ptr, p[1].data_->ptr, mean->ptr, rstd->ptr,
+                               o.grad_->ptr, 1.f, p[0].grad_->ptr, 1.f, p[1].grad_->ptr, p[2].grad_->ptr, nullptr),
+       "layernorm_bwd");
+  });
+}
+
+std::vector<Tensor> LayerNorm::parameters() const { return {weight, bias}; }
+
+Tensor relative_position_bias(const Tensor& table, size_t max_distance, bool bidirectional) {
+  require(table.shape.size() == 2, "relative_position_bias: the table is [buckets, heads]");
+  const int buckets = (int)table.shape[0], heads = (int)table.shape[1], far = (int)max_distance, both = bidirectional;
+  Tensor out = fresh({table.shape[1], 2 * max_distance + 1});
+  ok(talos_relpos_bias_fwd_f32(buckets, heads, far, both, table.data_->ptr, out.data_->ptr, nullptr, nullptr),
+     "relpos_bias_fwd");
+  return with_ctx(out, {table}, [=](const Tensor& o, std::vector<Tensor>& p) {
+    ok(talos_relpos_bias_bwd_f32(buckets, heads, far, both, o.grad_->ptr, 1.f, p[0].grad_->ptr, nullptr),
+       "relpos_bias_bwd");
+  });
+}
+
+namespace {
+
+// 32-bit whole numbers in a buffer of their own (a Storage's elements are as wide)
+std::shared_ptr<Storage> upload(const std::vector<int32_t>& v) {
+  auto s = std::make_shared<Storage>(v.size());
+  static_assert(sizeof(int32_t) == sizeof(float), "lengths and actions share Storage");
+  if (!v.empty()) ok(talos_memcpy_h2d(s->ptr, v.data(), v.size() * sizeof(int32_t), nullptr), "memcpy_h2d");
+  return s;
+}
+std::shared_ptr<Storage> upload(const std::vector<double>& v) {
+  auto s = std::make_shared<Storage>(v.size());
+  if (!v.empty()) ok(talos_memcpy_h2d_f64(s->ptr, v.data(), v.size(), nullptr), "memcpy_h2d_f64");
+  return s;
+}
+// grad += factor * from
+void add_into(const Tensor& t, const Storage& from, float factor) {
+  ok(talos_unary_bwd_f32(TALOS_SCALE, from.n, factor, 0.f, from.ptr, from.ptr, t.grad_->ptr, nullptr), "add_into");
+}
+
+}  // namespace
+
+Tensor grouped_attention(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, const Tensor* bias,
+                         const std::vector<int32_t>& q_lens, const std::vector<int32_t>& k_lens, double scale) {
+  require(q.shape.size() == 4 && k.shape.size() == 4 && v.shape.size() == 4, "grouped_attention: [b, s, heads, d] tensors");
+  const Shape &a = q.shape, &b = k.shape, &c = v.shape;
+  require(a[0] == b[0] && a[0] == c[0] && b[1] == c[1] && b[2] == c[2] && a[3] == b[3],
+          "grouped_attention: q " + shape_str(a) + ", k " + shape_str(b) + ", v " + shape_str(c));
+  require(!bias || (bias->shape.size() == 2 && bias->shape[0] == a[2] && bias->shape[1] % 2 == 1 && bias->shape[1] > 1),
+          "grouped_attention: the bias is [heads, 2 M + 1]");
+  require((q_lens.empty() || q_lens.size() == a[0]) && (k_lens.empty() || k_lens.size() == a[0]),
+          "grouped_attention: one length a sample");
+  talos_gqa_cfg cfg{};
+  cfg.batch = (int)a[0];
+  cfg.q_len = (int)a[1];
+  cfg.k_len = (int)b[1];
+  cfg.heads = (int)a[2];
+  cfg.kv_heads = (int)b[2];
+  cfg.qk_dim = (int)a[3];
+  cfg.v_dim = (int)c[3];
+  cfg.causal = causal;
+  cfg.max_distance = bias ? (int)(bias->shape[1] / 2) : 0;
+  cfg.scale = (float)(scale != 0.0 ? scale : 1.0 / std::sqrt((double)a[3]));
+  std::shared_ptr<Storage> ql = q_lens.empty() ? nullptr : upload(q_lens), kl = k_lens.empty() ? nullptr : upload(k_lens);
+  auto lens = [](const std::shared_ptr<Storage>& s) { return s ? reinterpret_cast<const int32_t*>(s->ptr) : nullptr; };
+  const long long lq = a[2] * a[3], lk = b[2] * b[3], lv = c[2] * c[3], lo = a[2] * c[3];
+  Tensor out = fresh({a[0], a[1], a[2], c[3]});
+  auto lse = std::make_shared<Storage>(a[0] * a[1] * a[2]);
+  ok(talos_gqa_fwd_f32(&cfg, lens(ql), lens(kl), bias ? bias->data_->ptr : nullptr, q.data_->ptr, lq, k.data_->ptr, lk,
+                       v.data_->ptr, lv, out.data_->ptr, lo, lse->ptr, nullptr),
+     "gqa_fwd");
+  std::vector<Tensor> parents{q, k, v};
+  if (bias) parents.push_back(*bias);
+  return with_ctx(out, parents, [=](const Tensor& o, std::vector<Tensor>& p) {
+    // the entry overwrites its gradients, the tape adds
+    Storage dq(p[0].numel()), dk(p[1].numel()), dv(p[2].numel());
+    const bool biased = p.size() > 3;
+    ok(talos_gqa_bwd_f32(&cfg, lens(ql), lens(kl), biased ? p[3].data_->ptr : nullptr, p[0].data_->ptr, lq,
+                         p[1].data_->ptr, lk, p[2].data_->ptr, lv, o.data_->ptr, lo, lse->ptr, o.grad_->ptr, lo, dq.ptr,
+                         lq, dk.ptr, lk, dv.ptr, lv, 1.f, biased ? p[3].grad_->ptr : nullptr, nullptr),
+       "gqa_bwd");
+    add_into(p[0], dq, 1.f);
+    add_into(p[1], dk, 1.f);
+    add_into(p[2], dv, 1.f);
+  });
+}
+
+Tensor policy_loss(const Tensor& logits, const PolicyBatch& batch, double clip_low, double clip_high, double kl_coef) {
+  require(logits.shape.size() == 2, "policy_loss: logits are [rows, vocab]");
+  const size_t rows = logits.shape[0], vocab = logits.shape[1];
+  require(batch.actions.size() == rows && batch.adv.size() == rows && batch.old_logp.size() == rows &&
+              (batch.ref_logp.empty() || batch.ref_logp.size() == rows) &&
+              (batch.weight.empty() || batch.weight.size() == rows),
+          "policy_loss: one value a row");
+  auto act = upload(batch.actions);
+  auto adv = upload(batch.adv), old = upload(batch.old_logp);
+  std::shared_ptr<Storage> ref = batch.ref_logp.empty() ? nullptr : upload(batch.ref_logp);
+  std::shared_ptr<Storage> weight = batch.weight.empty() ? nullptr : upload(batch.weight);
+  auto ptr = [](const std::shared_ptr<Storage>& s) { return s ? s->ptr : nullptr; };
+  Tensor out = fresh({1});
+  ok(talos_policy_loss_fwd_f32((int)rows, (int)vocab, (float)clip_low, (float)clip_high, (float)kl_coef,
+                               logits.data_->ptr, (long long)vocab, reinterpret_cast<const int32_t*>(act->ptr), adv->ptr,
+                               old->ptr, ptr(ref), ptr(weight), out.data_->ptr, nullptr, nullptr, 0, nullptr),
+     "policy_loss_fwd");
+  return with_ctx(out, {logits}, [=](const Tensor& o, std::vector<Tensor>& p) {
+    Storage d(p[0].numel());
+    ok(talos_policy_loss_bwd_f32((int)rows, (int)vocab, (float)clip_low, (float)clip_high, (float)kl_coef,
+                                 p[0].data_->ptr, (long long)vocab, reinterpret_cast<const int32_t*>(act->ptr), adv->ptr,
+                                 old->ptr, ptr(ref), ptr(weight), d.ptr, (long long)vocab, nullptr, nullptr, nullptr, 0,
+                                 nullptr),
+       "policy_loss_bwd");
+    add_into(p[0], d, (float)o.grad()[0]);
+  });
+}
+
+// ---------------------------------------------------------------------------
 // Attention ops (src/transformer.rs:877-1183)
 // ---------------------------------------------------------------------------
 // S[b] = Q[b] . K[b]^T on [b, seq, dim] buffers (batched_matmul_qt_k, :877-958): the batched GEMM

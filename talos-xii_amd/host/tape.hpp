@@ -16,6 +16,7 @@
 //   scale_tensor, softmax, concat_last_dim
 //   RoPE, MLAConfig, MultiHeadLatentAttention, LuckTransformer  same names (src/transformer.rs)
 //   Adam::new(params, lr) / step / zero_grad  Adam(params, lr[, max_grad_norm]) / step / zero_grad
+//   (none)                                    LayerNorm, relative_position_bias, grouped_attention, policy_loss
 //
 // Semantics kept: grads accumulate (+=) and only zero_grad clears them; backward() seeds every
 // element of the root's grad with 1.0 and runs the closures in reverse DFS topological order,
@@ -155,6 +156,35 @@ Tensor scale_tensor(const Tensor& t, double scale);
 Tensor softmax(const Tensor& t, size_t seq_len, bool causal = false);
 // [.., ca] ++ [.., cb] -> [.., ca + cb] (concat_last_dim, :1123-1183)
 Tensor concat_last_dim(const Tensor& a, const Tensor& b);
+
+// ---------------------------------------------------------------------------------------------
+// Operators of policies over long histories (extensions, no reference counterparts)
+// ---------------------------------------------------------------------------------------------
+// Layer norm over the last dimension: y = (x - mean) / sqrt(var + eps) * weight + bias (gain 1, bias 0 at first)
+struct LayerNorm : Module {
+  Tensor weight, bias;
+  double eps = 1e-5;
+  explicit LayerNorm(size_t dim, double eps = 1e-5);
+  Tensor forward(const Tensor& x) const override;
+  std::vector<Tensor> parameters() const override;
+};
+// table [buckets, heads] -> bias by distance [heads, 2 max_distance + 1] (talos_relpos_bias_fwd_f32's buckets)
+Tensor relative_position_bias(const Tensor& table, size_t max_distance, bool bidirectional);
+// q [b, q_len, heads, dk], k [b, k_len, kv_heads, dk], v [b, k_len, kv_heads, dv] -> [b, q_len, heads, dv]: attention
+// of any length, heads / kv_heads query heads on each key head, queries and keys of a sample ending together
+// (talos_gqa_fwd_f32). bias: a bias by distance [heads, 2 M + 1] (M <= 512), or null. q_lens, k_lens: each sample's
+// own lengths, or empty for the whole ones. scale 0 selects 1 / sqrt(dk).
+Tensor grouped_attention(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, const Tensor* bias = nullptr,
+                         const std::vector<int32_t>& q_lens = {}, const std::vector<int32_t>& k_lens = {},
+                         double scale = 0.0);
+// What the rows of a clipped policy loss are weighed by, one value a row (talos_policy_loss_fwd_f32): ref_logp empty
+// for no KL term, weight empty for 1 / rows each.
+struct PolicyBatch {
+  std::vector<int32_t> actions;
+  std::vector<double> adv, old_logp, ref_logp, weight;
+};
+// logits [rows, vocab] -> the loss [1]
+Tensor policy_loss(const Tensor& logits, const PolicyBatch& batch, double clip_low, double clip_high, double kl_coef);
 
 // RoPE (src/transformer.rs:219-337): interleaved pairs (2i, 2i+1) of the last dimension rotated by
 // pos * base^(-2i/dim), pos = start_pos + the index along shape[-2]; the cos / sin table is

@@ -8,7 +8,18 @@ probabilistic constant 32 for m (chains of up to 1000 terms) beside 8 u of the v
 """
 import math
 
+import pytest
 import torch
+
+
+@pytest.fixture(autouse=True)
+def float32_default():
+    """The sizes of the buffers made here do not depend on the default that another test module set."""
+    kept = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float32)
+    yield
+    torch.set_default_dtype(kept)
+
 
 U32, U16 = 2.0 ** -24, 2.0 ** -8
 

@@ -9,6 +9,7 @@ import torch
 
 import operators_ref as ref
 import talos_hip as th
+from operators_ref import float32_default  # noqa: F401
 
 P16 = ctypes.c_void_p(16)  # never dereferenced: the arguments' checks fail first
 DT = {"f32": torch.float32, "bf16": torch.bfloat16}
