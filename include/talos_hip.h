@@ -84,9 +84,10 @@ int talos_event_destroy(void* ev);
 int talos_event_record(void* ev, talos_stream_t stream);
 int talos_event_elapsed_ms(void* start, void* stop, float* ms);
 /* Caller-owned scratch for the kernel-level entry points called from this thread: the split-K
- * partials of the GEMMs, the D rows of talos_attn_bwd_f32 and the f64 partial sums of the
+ * partials of the GEMMs, the D rows of talos_attn_bwd_f32, the f64 partial sums of the
  * reductions (talos_bias_grad_f32, talos_rmsnorm_bwd_f32, talos_reduce_sum_f32,
- * talos_grad_sumsq_f32 with a NULL workspace). A call whose scratch fits the bound buffer uses it
+ * talos_grad_sumsq_f32 with a NULL workspace), the partial sums of talos_layernorm_bwd_* and
+ * talos_policy_loss_*, and the D rows and joined parts of talos_gqa_*. A call whose scratch fits the bound buffer uses it
  * and allocates nothing; a GEMM whose split-K partials would not fit splits K fewer times (down to
  * no split) instead; any other call that needs more allocates and frees on its stream
  * (hipMallocAsync / hipFreeAsync), as every call does when nothing is bound. ptr must be device
@@ -151,15 +152,17 @@ int talos_rmsnorm_bwd_f32(int rows, int dim, const float* x, const float* w, con
  * 1 / sqrt(var + eps). x and y are contiguous [rows, dim] at any element alignment; w [dim] and b
  * [dim] (b may be NULL: no bias) are fp32. Saves mean[rows] and rstd[rows] for the backward (either
  * may be NULL). The _bf16 entries take bf16 x, y, dy and dx; statistics, sums and the parameters'
- * gradients are fp32, and a bf16 result is rounded once. dim <= 2^26. y may be x. */
+ * gradients are fp32, and a bf16 result is rounded once. dim <= 2^26. y may be x; otherwise no output may
+ * overlap an input. */
 int talos_layernorm_fwd_f32(int rows, int dim, float eps, const float* x, const float* w, const float* b, float* y,
                             float* mean, float* rstd, talos_stream_t stream);
 int talos_layernorm_fwd_bf16(int rows, int dim, float eps, const talos_bf16* x, const float* w, const float* b,
                              talos_bf16* y, float* mean, float* rstd, talos_stream_t stream);
 /* Its backward: with xh = (x - mean) * rstd and h = dy * w, dx = beta_dx dx + rstd * (h - mean(h) -
  * xh * mean(h * xh)), dw = beta_dw dw + sum_rows dy * xh, db = beta_dw db + sum_rows dy (partial sums
- * added in f64, deterministic). dw and db may each be NULL; dx may be dy. Scratch: up to 512 partial
- * rows of 2 dim floats (talos_workspace_bind). */
+ * added in f64, deterministic). dw and db may each be NULL; dx may be dy, and no other output may overlap
+ * an input. Scratch (talos_workspace_bind), where dw or db is wanted: at most 512 partial rows of 2 dim
+ * floats. */
 int talos_layernorm_bwd_f32(int rows, int dim, const float* x, const float* w, const float* mean, const float* rstd,
                             const float* dy, float beta_dx, float* dx, float beta_dw, float* dw, float* db,
                             talos_stream_t stream);
@@ -225,21 +228,25 @@ int talos_attn_bwd_noalloc_f32(int batch, int seq, int heads, int qk_dim, int v_
  * o [batch, q_len, heads, v_dim], with row strides ld_* (elements between consecutive tokens; sample b
  * begins at row b * q_len or b * k_len), at any element alignment; lse[batch, heads, q_len] is fp32.
  * q_lens, k_lens: device int32[batch] (NULL: all q_len, k_len), clamped to [0, q_len] and [0, k_len].
- * Rows past a sample's length are not read (they may hold anything). The queries and keys of a sample
+ * Rows past a sample's length are not read (they may hold anything); a key within it that the causal
+ * mask hides from a query must be finite, as 0 times its value still enters that query's sum. The queries and keys of a sample
  * end together: query i stands at position i + k_lens[b] - q_lens[b], so the same call serves whole
  * sequences, a chunk of new tokens or a single one after a cache, and a causal query sees the keys j
  * <= its position.
  *   s_ij = scale q_i . k_j + bias[h, clamp(j - position_i, -M, M) + M],   o_i = sum_j softmax_j(s_i) v_j,
  *   lse_i = ln sum_j exp(s_ij)
  * bias: fp32 [heads, 2 M + 1], M = max_distance, or NULL (talos_relpos_bias_fwd_f32 makes one from a
- * table by buckets). A query that sees no key, and every row past q_lens[b], gets o = 0 and lse =
- * -infinity.
+ * table by buckets); an entry of -infinity, or below -3.4e30 (the type's lowest value), hides the keys at
+ * its distance. A query that sees no key, and every row past q_lens[b], gets o = 0 and lse = -infinity.
  *
  * talos_gqa_fwd_f32 / _bwd_f32 take fp32 tensors and products of three-piece bf16 splits (fp32
  * accuracy, as talos_gemm_f32; values past 3.39e38 give NaN, and bits of a product below 2^-133 are
  * lost); the _bf16 entries take bf16 q, k, v, o and their gradients, with fp32 scores, softmax and
  * accumulators, the probabilities and their gradients rounded to bf16 as operands.
- * qk_dim, v_dim <= 128. batch * heads <= 65535 and a sample's stride is not limited to 32 bits. */
+ * qk_dim, v_dim <= 128; q_len * heads, k_len and batch * heads <= 2^30 (addresses are 64 bits wide);
+ * 1e-30 <= scale <= 1e30; 1 <= max_distance <= 2^20. No output may overlap an input. Scratch
+ * (talos_workspace_bind): where few rows leave the device idle, the keys are cut into parts, whose fp32
+ * results are joined (at most a workgroup's rows for each of 1024 workgroups). */
 typedef struct talos_gqa_cfg {
   int batch;
   int q_len;
@@ -260,7 +267,8 @@ int talos_gqa_fwd_bf16(const talos_gqa_cfg* cfg, const int32_t* q_lens, const in
                        long long ld_v, talos_bf16* o, long long ld_o, float* lse, talos_stream_t stream);
 /* Its backward from o and lse of the forward: dq, dk, dv are overwritten (zero past the lengths; the
  * heads of a group add into their shared key head), and dbias = beta_bias dbias + the scores'
- * gradients summed by distance, when bias is given and dbias is not NULL (M <= 512). Every sum has a
+ * gradients summed by distance, when bias is given and dbias is not NULL (M <= 512, heads <= 65535). lens,
+ * bias and lse must be the forward's. Every sum has a
  * fixed order: no atomics, the same bits on every call. Scratch (talos_workspace_bind): the rows'
  * D = rowsum(dout * o) and, where the work is split, partial sums. */
 int talos_gqa_bwd_f32(const talos_gqa_cfg* cfg, const int32_t* q_lens, const int32_t* k_lens, const float* bias,
@@ -536,7 +544,7 @@ int talos_ppo_head_loss_bwd_f32(int n, int n_actions, float clip_eps, float valu
  * ref_logp may be NULL (no KL term, kl_coef 0); weight may be NULL: 1 / rows each. A row of weight 0 is
  * padding: its logits and scalars are not used, its logp and gradient are 0. A logit of -infinity is an
  * action that cannot be taken (the taken one must be finite). An action outside [0, vocab) makes the
- * loss NaN, with a zero gradient. loss (device float[1]), logp (float[rows]) and stats (device
+ * loss NaN, with a zero gradient (that row's logp is NaN). loss (device float[1]), logp (float[rows]) and stats (device
  * double[TALOS_POLICY_NSTATS], sums over the rows of non-zero weight, added into when
  * stats_accumulate != 0) may each be NULL, the forward's not all. vocab <= 2^26. */
 enum talos_policy_stat {

@@ -256,6 +256,11 @@ __device__ __forceinline__ float gq_sum_halves(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// A bias entry in units of log 2. The product overflows below -3.4e30, so such an entry (the type's lowest value, as masks
+// are often written) hides its keys as -infinity does: where a row's every key had one, no digits of lse would be left to
+// form its probabilities from again.
+__device__ __forceinline__ float gq_bias(float b) { return b * 1e8f * (kLog2e * 1e-8f); }
+
 // A sample's lengths and where its queries stand among its keys.
 struct GqaSample {
   int ql, kl, off;

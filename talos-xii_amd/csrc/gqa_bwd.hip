@@ -8,7 +8,7 @@
 //   dQ^T += K^T dS^T, with dS^T straight from the accumulator.
 // * dK and dV: a wave holds 32 keys and walks the queries of the group's heads, one head after the other:
 //   S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS. The heads of a group add into the same registers.
-// That is seven block products where one kernel with atomic dQ would need five.
+// That is seven block products (eight for bf16, below) where one kernel that adds dQ atomically would need five.
 //
 // D of a bf16 o. The forward's o carries the rounding of its probabilities and its own, 2^-9 of o each, and D from it is
 // off by that share of dO o: nothing to dQ and dK of long even rows, but of a row that sees few keys (or looks at few) o is
@@ -115,8 +115,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
   const int pos = qi + sm.off;
   if (BIAS) {
     bias = a.bias + (size_t)(live ? head : 0) * (2 * a.M + 1) + a.M;
-    bias_l = bias[-a.M] * kLog2e;
-    bias_r = bias[a.M] * kLog2e;
+    bias_l = gq_bias(bias[-a.M]);
+    bias_r = gq_bias(bias[a.M]);
   }
 
   GqaLane<D> ln;
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int d = k0 + gq_row(r, h) - pos;
-            s[r] = fmaf(s[r], a.c, bias[min(max(d, -a.M), a.M)] * kLog2e);
+            s[r] = fmaf(s[r], a.c, gq_bias(bias[min(max(d, -a.M), a.M)]));
           }
         }
       }
@@ -430,8 +430,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
     float bias_l = 0.f, bias_r = 0.f, far_l = 0.f, far_r = 0.f;
     if (BIAS) {
       bias = a.bias + (size_t)head * (2 * a.M + 1) + a.M;
-      bias_l = bias[-a.M] * kLog2e;
-      bias_r = bias[a.M] * kLog2e;
+      bias_l = gq_bias(bias[-a.M]);
+      bias_r = gq_bias(bias[a.M]);
     }
     float* mine = dist + wv * W + a.M + kSlack;
     if (BIAS == 2) {
@@ -503,7 +503,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int d = key - (q0 + gq_row(r, h) + sm.off);
-              s[r] = fmaf(s[r], a.c, bias[min(max(d, -a.M), a.M)] * kLog2e);
+              s[r] = fmaf(s[r], a.c, gq_bias(bias[min(max(d, -a.M), a.M)]));
             }
           }
         }
@@ -642,7 +642,6 @@ __global__ __launch_bounds__(1024) void gqa_dbias_kernel(int B, int H, int per, 
 struct BwdShape {
   const void* dq[2];
   const void* dkv[3];
-  int nk, nq;
   size_t dq_lds;
   size_t (*dkv_lds)(bool, int);
 };
@@ -651,7 +650,7 @@ BwdShape bwd_shape() {
   return {{(const void*)gqa_dq_kernel<T, D, NK, NBK, false, DMA>, (const void*)gqa_dq_kernel<T, D, NK, NBK, true, DMA>},
           {(const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 0, DMA>, (const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 1, DMA>,
            (const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 2, DMA>},
-          NK, NQ, DqShape<T, D, NK, NBK>::lds, DkvShape<T, D, NQ, NBQ>::lds};
+          DqShape<T, D, NK, NBK>::lds, DkvShape<T, D, NQ, NBQ>::lds};
 }
 template <typename T>
 BwdShape pick_bwd(int d, bool dma) {

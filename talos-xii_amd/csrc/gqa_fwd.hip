@@ -105,8 +105,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
   const int pos = qi + sm.off;
   if (BIAS) {
     bias = a.bias + (size_t)(live ? head : 0) * (2 * a.M + 1) + a.M;
-    bias_l = bias[-a.M] * kLog2e;
-    bias_r = bias[a.M] * kLog2e;
+    bias_l = gq_bias(bias[-a.M]);
+    bias_r = gq_bias(bias[a.M]);
   }
 
   GqaLane<D> ln;
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int d = k0 + kb * 32 + gq_row(r, h) - pos;
-            s[kb][r] = fmaf(s[kb][r], a.c, bias[min(max(d, -a.M), a.M)] * kLog2e);
+            s[kb][r] = fmaf(s[kb][r], a.c, gq_bias(bias[min(max(d, -a.M), a.M)]));
           }
       }
     }

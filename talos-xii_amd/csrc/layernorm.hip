@@ -127,7 +127,8 @@ __global__ __launch_bounds__(kLnThreads<L>) void layernorm_fwd_kernel(int rows, 
   }
 }
 
-// Rows of any width: a workgroup a row, the row read three times (the second and third from cache).
+// Rows of any width: a workgroup a row, the row read three times (the second and third from cache). A lane's own sums,
+// up to 2^18 terms, are f64.
 template <typename T>
 __global__ __launch_bounds__(256) void layernorm_fwd_wide_kernel(int rows, int dim, float eps, const T* x,
                                                                  const float* __restrict__ w,
@@ -140,21 +141,21 @@ __global__ __launch_bounds__(256) void layernorm_fwd_wide_kernel(int rows, int d
   const T* xr = x + (size_t)row * dim;
   T* yr = y + (size_t)row * dim;
   const float inv = 1.0f / (float)dim;
-  float s = 0.f, q = 0.f;
+  double s = 0.0, q = 0.0;
   for (int c = N * threadIdx.x; c < dim; c += N * 256) {
     float v[N];
     load_piece(xr, c, dim, v);
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += v[i];
+    for (int i = 0; i < N; ++i) s += (double)v[i];
   }
-  const float mean = row_sum<256>(s, red) * inv;
+  const float mean = row_sum<256>((float)s, red) * inv;
   for (int c = N * threadIdx.x; c < dim; c += N * 256) {
     float v[N];
     load_piece(xr, c, dim, v);
 #pragma unroll
-    for (int i = 0; i < N; ++i) q += c + i < dim ? (v[i] - mean) * (v[i] - mean) : 0.f;
+    for (int i = 0; i < N; ++i) q += (double)(c + i < dim ? (v[i] - mean) * (v[i] - mean) : 0.f);
   }
-  const float rstd = 1.0f / sqrtf(row_sum<256>(q, red) * inv + eps);
+  const float rstd = 1.0f / sqrtf(row_sum<256>((float)q, red) * inv + eps);
   if (threadIdx.x == 0) {
     if (mean_out) mean_out[row] = mean;
     if (rstd_out) rstd_out[row] = rstd;
@@ -292,7 +293,7 @@ __global__ __launch_bounds__(kLnThreads<L>) void layernorm_bwd_kernel(int rows, 
   }
 }
 
-// dx of rows of any width: a workgroup a row, the row read twice.
+// dx of rows of any width: a workgroup a row, the row read twice; a lane's own sums f64.
 template <typename T>
 __global__ __launch_bounds__(256) void layernorm_bwd_wide_kernel(int rows, int dim, const T* __restrict__ x,
                                                                  const float* __restrict__ w,
@@ -305,7 +306,7 @@ __global__ __launch_bounds__(256) void layernorm_bwd_wide_kernel(int rows, int d
   const T *xr = x + (size_t)row * dim, *gr = dy + (size_t)row * dim;
   T* dr = dx + (size_t)row * dim;
   const float inv = 1.0f / (float)dim, m = mean[row], r = rstd[row];
-  float s = 0.f, q = 0.f;
+  double s64 = 0.0, q64 = 0.0;
   for (int c = N * threadIdx.x; c < dim; c += N * 256) {
     float v[N], g[N];
     load_piece(xr, c, dim, v);
@@ -313,12 +314,14 @@ __global__ __launch_bounds__(256) void layernorm_bwd_wide_kernel(int rows, int d
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float h = c + i < dim ? g[i] * w[c + i] : 0.f;
-      s += h;
-      q += h * ((v[i] - m) * r);
+      s64 += (double)h;
+      q64 += (double)(h * ((v[i] - m) * r));
     }
   }
-  s = row_sum<256>(s, red) * inv;
-  q = row_sum<256>(q, red) * inv;
+  float s = (float)s64, q = (float)q64;
+  row_sum2<256>(s, q, red);
+  s *= inv;
+  q *= inv;
   for (int c = N * threadIdx.x; c < dim; c += N * 256) {
     float v[N], g[N], o[N];
     load_piece(xr, c, dim, v);

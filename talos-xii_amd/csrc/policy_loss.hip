@@ -293,6 +293,8 @@ int policy_loss(const char* fn, int rows, int vocab, float clip_low, float clip_
   TALOS_REQUIRE(clip_low >= 0.f && clip_high >= 0.f, TALOS_ERR_SHAPE, "%s: clip_low and clip_high must be >= 0", fn);
   TALOS_REQUIRE(ld >= vocab && (!dlogits || ld_d >= vocab), TALOS_ERR_SHAPE, "%s: a row stride is smaller than vocab",
                 fn);
+  TALOS_REQUIRE(!dlogits || (const void*)dlogits != (const void*)logits || ld == ld_d, TALOS_ERR_SHAPE,
+                "%s: dlogits in the logits' place needs their row stride", fn);
   TALOS_REQUIRE(accumulate == 0 || accumulate == 1, TALOS_ERR_SHAPE, "%s: stats_accumulate must be 0 or 1", fn);
   TALOS_REQUIRE(rows == 0 || (logits && actions && adv && old_logp), TALOS_ERR_NULL, "%s: null input", fn);
   TALOS_REQUIRE(kl_coef == 0.f || ref_logp || rows == 0, TALOS_ERR_NULL, "%s: kl_coef without ref_logp", fn);

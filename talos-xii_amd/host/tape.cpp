@@ -42,8 +42,9 @@ void require(bool c, const std::string& msg) {
 
 // The scratch of the library calls made by this thread's ops (split-K partials, reduction
 // partials, attention rows): one device buffer bound on the thread's first op and held until the
-// thread exits, so an op never allocates scratch per call (a split-K product splits fewer times
-// rather than outgrow it). Every op runs on the null stream, so calls sharing it never overlap.
+// thread exits, so an op whose scratch fits allocates none per call (a split-K product splits fewer
+// times rather than outgrow it; the gradients of grouped_attention over long sequences do outgrow it
+// and take theirs from the stream's pool). Every op runs on the null stream, so calls sharing it never overlap.
 // A workspace the caller bound on this thread before its first op stays bound instead.
 constexpr size_t kTapeWorkspaceBytes = size_t(16) << 20;
 struct TapeWorkspace {

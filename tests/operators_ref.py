@@ -133,8 +133,12 @@ def attention(q, k, v, scale, causal, qlens, klens, bias=None, do=None):
             if bias is not None:
                 M = bias.shape[1] // 2
                 at = apart.clamp(-M, M) + M
-                s, sm = s + bias[h][at], sm + bias[h][at].abs()
+                hidden = bias[h][at] < -3.4e30  # such entries hide the keys at their distance
+                near = torch.where(hidden, 0.0, bias[h][at])
+                s, sm = s + near, sm + near.abs()
             see = apart <= 0 if causal else torch.ones_like(apart, dtype=torch.bool)
+            if bias is not None:
+                see = see & ~hidden
             some = see.any(1)
             s = s.masked_fill(~see, -math.inf)
             top = torch.where(some, s.max(1).values, 0.0)

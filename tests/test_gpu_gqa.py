@@ -186,6 +186,26 @@ def test_scores_of_any_size(ty):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.float32).min, -3.5e30])
+@pytest.mark.parametrize("causal", [0, 1])
+def test_distances_hidden_by_the_bias(causal, low, ty):
+    """Minus infinity and the type's lowest value hide a distance, on a block's edge, inside it and beyond M; rows that see
+    only hidden keys get nothing, and neither they nor those keys get a gradient from them."""
+    c = Case(ty, 2, 90, 190, 4, 2, 64, 64, causal, [90, 41], [190, 40], M=70, seed=11)
+    c.bias[0, ::2] = low
+    c.bias[1, 70] = low  # the query's own position; sample 1's second causal row sees nothing else
+    c.bias[2, 0] = low  # everything far behind
+    c.bias[3, 0], c.bias[3, 50:] = low, low
+    c.Bias.copy_(c.bias)
+    c.check()
+    c = Case(ty, 1, 5, 40, 2, 2, 32, 32, causal, M=3, seed=12)
+    c.bias[1] = low  # a head with nothing to see
+    c.Bias.copy_(c.bias)
+    c.check()
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences():
     c = Case("f32", 1, 7, 9, 2, 1, 8, 8, 1, M=3, seed=8)
     c.fwd()
@@ -287,6 +307,9 @@ def test_refusals():
         for scale in (0.0, -1.0, math.inf, math.nan):
             both(th.ERR_SHAPE, cfg(scale=scale))
         both(th.ERR_SHAPE, cfg(max_distance=0))
+        both(th.ERR_UNSUPPORTED, cfg(scale=1e-31))
+        both(th.ERR_UNSUPPORTED, cfg(scale=2e30))
+        assert fwd(cfg(max_distance=(1 << 20) + 1), None, None, P16, *base, None) == th.ERR_SHAPE
         both(th.ERR_UNSUPPORTED, cfg(q_len=1 << 29))
         both(th.ERR_UNSUPPORTED, cfg(batch=1 << 29))
         for i in (1, 3, 5, 7):

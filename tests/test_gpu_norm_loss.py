@@ -307,3 +307,4 @@ def test_policy_loss_refusals():
         assert fwd(4, (1 << 26) + 1, 0.2, 0.2, 0.1, P16, 1 << 27, *ins, P16, None, None, 0, None) == th.ERR_UNSUPPORTED
         assert bwd(4, 8, 0.2, 0.2, 0.1, P16, 8, *ins, None, 8, P16, None, None, 0, None) == th.ERR_NULL
         assert bwd(4, 8, 0.2, 0.2, 0.1, P16, 8, *ins, P16, 5, P16, None, None, 0, None) == th.ERR_SHAPE
+        assert bwd(4, 8, 0.2, 0.2, 0.1, P16, 12, *ins, P16, 8, P16, None, None, 0, None) == th.ERR_SHAPE  # in place, rows apart
