@@ -10,8 +10,8 @@
 // is rounded once, from its fp32 value.
 //
 // L lanes share a row, each holding V pieces of 16 bytes: 8, 16 or 32 lanes where a row has that few
-// pieces, a wave up to 2048 values, four waves up to 8192, and beyond that a loop that reads the row
-// again. The backward keeps every lane's column sums in registers over the rows that its workgroup
+// pieces, a wave up to 1024 values, more waves up to 8192 (pick_shape), and beyond that a loop that reads
+// the row again. The backward keeps every lane's column sums in registers over the rows that its workgroup
 // walks; the lanes and waves of a workgroup add theirs in LDS, and a second kernel adds the
 // workgroups' fp32 partial rows in f64, in a fixed order.
 #include <algorithm>
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(kLnThreads<L>) void layernorm_fwd_kernel(int rows, 
   auto fetch = [&](long long row) {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      next[j] = load_raw(x + (size_t)(row < rows ? row : 0) * dim, row < rows ? N * (lane + L * j) : dim, dim);
+      next[j] = row_piece(x + (size_t)(row < rows ? row : 0) * dim, N * (lane + L * j), dim);
   };
   const long long step = (long long)gridDim.x * R;
   fetch((long long)blockIdx.x * R + sub);
@@ -96,6 +96,7 @@ __global__ __launch_bounds__(kLnThreads<L>) void layernorm_fwd_kernel(int rows, 
     float s = 0.f, q = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
+      row_piece_end<T>(next[j], N * (lane + L * j), dim);
       Piece<T>::widen(next[j], v[j]);
 #pragma unroll
       for (int i = 0; i < N; ++i) s += v[j][i];
@@ -204,9 +205,9 @@ __global__ __launch_bounds__(kLnThreads<L>) void layernorm_bwd_kernel(int rows, 
     nr = on ? rstd[row] : 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = on ? N * (lane + L * j) : dim;
-      nx[j] = load_raw(x + (size_t)(on ? row : 0) * dim, c, dim);
-      ng[j] = load_raw(dy + (size_t)(on ? row : 0) * dim, c, dim);
+      const int c = N * (lane + L * j);
+      nx[j] = row_piece(x + (size_t)(on ? row : 0) * dim, c, dim);
+      ng[j] = row_piece(dy + (size_t)(on ? row : 0) * dim, c, dim);
     }
   };
   const long long step = (long long)gridDim.x * R;
@@ -219,6 +220,9 @@ __global__ __launch_bounds__(kLnThreads<L>) void layernorm_bwd_kernel(int rows, 
     float s = 0.f, q = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
+      const int c = on ? N * (lane + L * j) : dim;  // a row past the last: zeros
+      row_piece_end<T>(nx[j], c, dim);
+      row_piece_end<T>(ng[j], c, dim);
       Piece<T>::widen(nx[j], xh[j]);
       Piece<T>::widen(ng[j], g[j]);
     }
@@ -384,15 +388,19 @@ __global__ __launch_bounds__(1024) void layernorm_parts_kernel(int dim, int npar
   if (o) *o = (float)(s + (beta != 0.f ? (double)*o : 0.0));
 }
 
-// Workgroups of the backward: two a compute unit hold the rows in flight that memory needs, and each
-// writes one partial row.
+// Workgroups of the backward, each of which writes one partial row: two a compute unit (8192 x 4096 bf16, forward and
+// backward, 69 us; one 87, four 84), one where a row takes more than eight waves, of which no second set fits beside it
+// (4096 x 8192 bf16, backward: 42 us; 53 with two in turn).
 constexpr int kLnBlocks = 512;
 constexpr int kLnWideParts = 64;
 constexpr int kLnMaxDim = 1 << 26;
 
-// f(L, V) with the lanes a row and the pieces a lane for `dim`: 16 values a lane at most, which the backward holds beside
-// another row's and two sums a column; false beyond 8192 values.
-template <typename T, typename F>
+// f(L, V) with the lanes a row and the pieces a lane for `dim`; false beyond 8192 values. 16 values a lane at most, which
+// the backward holds beside another row's and two sums a column; past 4096 values it takes 8 a lane for bf16 and fp32 alike
+// (4377 bf16: 58 us, 88 with 16 in half as many lanes), the forward 16 (33 us, 42 with 8). A row of 257 to 384 pieces
+// leaves fewer lanes idle in six waves: backward of 2500 bf16 50 us, 55 with four waves of twice the pieces (the
+// forward 49, 30 with four).
+template <typename T, bool BWD, typename F>
 bool pick_shape(int dim, F&& f) {
   constexpr int N = Piece<T>::N, U = N == 4 ? 2 : 1;
   const int pieces = (dim + N - 1) / N;
@@ -408,18 +416,28 @@ bool pick_shape(int dim, F&& f) {
   TALOS_LN_SHAPE(64, 2)
   if constexpr (N == 4) TALOS_LN_SHAPE(64, 4)
   TALOS_LN_SHAPE(256, U)
+  if constexpr (BWD) TALOS_LN_SHAPE(384, U)
   TALOS_LN_SHAPE(256, 2 * U)
-  TALOS_LN_SHAPE(1024, U)
+  if constexpr (BWD) {
+    TALOS_LN_SHAPE(768, U)
+    TALOS_LN_SHAPE(1024, U)
+  } else {
+    TALOS_LN_SHAPE(512, 2 * U)
+  }
 #undef TALOS_LN_SHAPE
   return false;
 }
 
 template <typename T>
 int bwd_blocks(int rows, int dim) {
-  int per = 1;
-  const bool held = pick_shape<T>(dim, [&](auto L, auto) { per = kLnThreads<decltype(L)::value> / decltype(L)::value; });
+  int per = 1, most = kLnBlocks;
+  const bool held = pick_shape<T, true>(dim, [&](auto L, auto) {
+    constexpr int kL = decltype(L)::value;
+    per = kLnThreads<kL> / kL;
+    if (kL > 512) most = kLnBlocks / 2;
+  });
   if (!held) return std::min<int>(kLnWideParts, (int)ceil_div(rows, 4));
-  return std::min<int>(kLnBlocks, (int)ceil_div(rows, per));
+  return std::min<int>(most, (int)ceil_div(rows, per));
 }
 
 template <typename T>
@@ -431,9 +449,9 @@ int layernorm_fwd(const char* fn, int rows, int dim, float eps, const T* x, cons
   TALOS_REQUIRE(dim <= kLnMaxDim, TALOS_ERR_UNSUPPORTED, "%s: dim %d exceeds %d", fn, dim, kLnMaxDim);
   TALOS_DEVICE();
   if (rows == 0) return entry_done(TALOS_OK, s);
-  const bool held = pick_shape<T>(dim, [&](auto L, auto V) {
+  const bool held = pick_shape<T, false>(dim, [&](auto L, auto V) {
     constexpr int kL = decltype(L)::value, kV = decltype(V)::value;
-    // half of what the device holds at once: 1024 threads a compute unit
+    // 1024 threads a compute unit, half of what it holds: the rest of its registers are the rows on their way
     constexpr int kThreads = kLnThreads<kL>;
     const unsigned blocks = std::min<unsigned>(ceil_div(rows, kThreads / kL), 128 * 2048 / kThreads);
     hipLaunchKernelGGL((layernorm_fwd_kernel<T, kL, kV>), dim3(blocks), dim3(kThreads), 0, s, rows, dim, eps, x, w, b, y,
@@ -461,9 +479,10 @@ int layernorm_bwd(const char* fn, int rows, int dim, const T* x, const float* w,
   if (rc) return rc;
   float* part = static_cast<float*>(ws.ptr);
   if (rows > 0) {
-    const bool held = pick_shape<T>(dim, [&](auto L, auto V) {
+    const bool held = pick_shape<T, true>(dim, [&](auto L, auto V) {
       constexpr int kL = decltype(L)::value;
-      hipLaunchKernelGGL((layernorm_bwd_kernel<T, kL, decltype(V)::value>), dim3(nblk), dim3(kLnThreads<kL>), 0, s, rows, dim, x, w, mean, rstd, dy, beta_dx != 0.f, dx, part);
+      hipLaunchKernelGGL((layernorm_bwd_kernel<T, kL, decltype(V)::value>), dim3(nblk), dim3(kLnThreads<kL>), 0, s,
+                         rows, dim, x, w, mean, rstd, dy, beta_dx != 0.f, dx, part);
     });
     if (!held) {
       // the column sums first: dx may be dy's own buffer

@@ -85,6 +85,37 @@ __device__ __forceinline__ typename Piece<T>::Raw load_raw(const T* row, int c, 
   load_piece(row, c, dim, v, fill);
   return Piece<T>::pack(v);
 }
+// The same in two steps, so that the loads of many pieces are in flight together and none is waited for where it is issued
+// (a piece across the end, loaded value by value, is): row_piece loads the piece, or the row's last N values where it would
+// pass its end; row_piece_end moves those into place, `fill` behind them. (13421 rows of 2500 bf16 values, layer norm
+// forward and backward: 40 + 87 us with load_raw, 30 + 50 so; 7666 of 4377: 42 + 83, 33 + 58.)
+template <typename T>
+__device__ __forceinline__ typename Piece<T>::Raw row_piece(const T* row, int c, int dim, float fill = 0.f) {
+  if (dim < Piece<T>::N) return load_raw(row, c, dim, fill);
+  return *reinterpret_cast<const typename Piece<T>::Raw*>(row + min(c, dim - Piece<T>::N));
+}
+template <typename T>
+__device__ __forceinline__ void row_piece_end(typename Piece<T>::Raw& r, int c, int dim, float fill = 0.f) {
+  constexpr int N = Piece<T>::N, P = N / 4;  // values a piece, a word
+  const int over = c + N - dim;              // values past the end
+  if (over <= 0) return;
+  const uint32_t none = P == 1 ? __float_as_uint(fill) : bf16_round2(fill, fill);
+  auto words = [&](int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = i + n < 4 ? r.w[(i + n) & 3] : none;
+  };
+  if (over >= N) {
+    words(4);
+    return;
+  }
+  if (dim < N) return;
+  if (over & (2 * P)) words(2);
+  if (over & P) words(1);
+  if (P == 2 && (over & 1)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = r.w[i] >> 16 | (i < 3 ? r.w[(i + 1) & 3] : none) << 16;
+  }
+}
 template <typename T>
 __device__ __forceinline__ void store_piece(T* row, int c, int dim, const float (&v)[Piece<T>::N]) {
   constexpr int N = Piece<T>::N;
