@@ -12,8 +12,9 @@
 // the registers), its maximum, its sum of exponentials and the taken logit are formed, and the gradient
 // is written from the same registers: one read and one write of the logits for loss and gradient
 // together. L lanes hold a row, V pieces each: 8 lanes up to 32 (fp32) or 64 (bf16) actions, a wave
-// up to 2048 or 4096, four waves or sixteen beyond, up to 16384 fp32 or 32768 bf16 columns; wider rows are read again. The sums
-// are fp32 (at most a few dozen terms a lane, then a tree).
+// up to 2048 or 4096, four waves or sixteen beyond, up to 16384 fp32 or 32768 bf16 columns; wider rows are
+// read again. The
+// exponentials are fp32 (f64 in rows of a few values), their sums f64 from a piece on.
 //
 // Rows of weight 0 are padding: their logits are not read, their gradient is zero.
 #include <algorithm>
@@ -28,8 +29,8 @@ namespace {
 // partial sums of a workgroup: the loss, then the entries of enum talos_policy_stat
 constexpr int kPolParts = 1 + TALOS_POLICY_NSTATS;
 // 16-byte pieces of a row that sixteen waves hold (4 a lane). With 8 a lane a compute unit no longer has room for two
-// workgroups, and reading the row again, from cache, is faster: 2048 x 30001 fp32 138 -> 130 us, x 40000 bf16 114 -> 82;
-// with 4, holding is: 4096 x 32768 bf16 136 -> 119 us.
+// workgroups, and reading the row again, from cache, is faster: 2048 x 30001 fp32 138 -> 130 us, x 40000 bf16 114 -> 83;
+// with 4, holding is: 4096 x 32768 bf16 136 -> 117 us.
 constexpr int kHeld = 4096;
 constexpr int kPolicyMaxVocab = 1 << 26;
 
@@ -50,48 +51,110 @@ struct RowTerms {
   float slope, logp;
 };
 
-// exp(g) - g - 1: by its series near 0, where the difference would keep few digits
-__device__ __forceinline__ float exp_rest(float g) {
-  if (fabsf(g) < 0.25f) {
-    // 1/2 + g (1/6 + g (1/24 + ...)), the term left out below 2^-25 of the first
-    const float p = fmaf(g, fmaf(g, fmaf(g, fmaf(g, fmaf(g, 1.f / 5040.f, 1.f / 720.f), 1.f / 120.f), 1.f / 24.f), 1.f / 6.f), 0.5f);
-    return g * g * p;
+// A row's scalars are f64: gains of either sign cancel in the loss (to a hundredth of their size over a minibatch), and
+// so do ratio - 1 and its logarithm. The library's f64 exp, expm1 and log cost 400 instructions a row between them, a third of
+// the time of rows of 3000 bf16 values; these are a fifth of it, to 2^-41 (8192 x 2999 bf16: 32.4 us, with fp32 functions
+// and sums 30.1, whose loss was 10 to 100 times less exact; 4096 x 32768 bf16 117 us, 115).
+struct Exp {
+  double value, less, rest;  // exp(d), exp(d) - 1, exp(d) - 1 - d
+};
+// 2^n exp(r) with |r| <= ln 2 / 2, exp(r) = 1 + r + r^2 (1/2 + r/6 + ... + r^8/10!): the next term is below 2^-42
+__device__ __forceinline__ Exp exp_f64(double d) {
+  const double held = fmin(fmax(d, -2000.0), 2000.0);
+  const double n = rint(held * 1.4426950408889634);
+  // ln 2 in two parts, the first of 31 bits, so that n times it is exact
+  constexpr double kHi = 1488522236.0 / 2147483648.0, kLo = -4.2009150726810846e-11;
+  const double r = fma(n, -kLo, fma(n, -kHi, held));
+  double q = 1.0 / 3628800.0;
+  q = fma(q, r, 1.0 / 362880.0);
+  q = fma(q, r, 1.0 / 40320.0);
+  q = fma(q, r, 1.0 / 5040.0);
+  q = fma(q, r, 1.0 / 720.0);
+  q = fma(q, r, 1.0 / 120.0);
+  q = fma(q, r, 1.0 / 24.0);
+  q = fma(q, r, 1.0 / 6.0);
+  q = fma(q, r, 0.5);
+  q = q * r * r;
+  Exp e;
+  e.value = d != d ? d : ldexp(q + r + 1.0, (int)n);
+  e.less = n == 0.0 ? q + r : e.value - 1.0;
+  e.rest = n == 0.0 ? q : e.less - d;
+  return e;
+}
+// log z = n ln 2 + 2 atanh((m - 1) / (m + 1)), m within sqrt(1/2) .. sqrt(2): the term left out is below 2^-44
+__device__ __forceinline__ double log_f64(double z) {
+  int n;
+  double m = frexp(z, &n);
+  if (m < 0.70710678118654752) {
+    m += m;
+    --n;
   }
-  return expm1f(g) - g;
+  const double s = (m - 1.0) / (m + 1.0), t = s * s;
+  double p = 2.0 / 15.0;
+  p = fma(p, t, 2.0 / 13.0);
+  p = fma(p, t, 2.0 / 11.0);
+  p = fma(p, t, 2.0 / 9.0);
+  p = fma(p, t, 2.0 / 7.0);
+  p = fma(p, t, 2.0 / 5.0);
+  p = fma(p, t, 2.0 / 3.0);
+  p = fma(p, t, 2.0);
+  return fma((double)n, 0.69314718055994531, p * s);
 }
 
 // From the row's maximum, the sum of its exponentials and the taken logit. An action out of range has no
-// log-probability: a NaN loss and no gradient. Log-probabilities and their differences are f64, as the clip's border is
-// looked up in them; the exponentials of the differences are fp32 (the f64 functions, 400 instructions a row and their
-// constants, took a third of the time of rows of 3000 bf16 values).
-__device__ __forceinline__ RowTerms policy_row(const PolicyArgs& a, int row, bool bad, float top, float sum,
+// log-probability: a NaN loss and no gradient.
+__device__ __forceinline__ RowTerms policy_row(const PolicyArgs& a, int row, bool bad, float top, double sum,
                                                float taken) {
   RowTerms t;
   const double w = a.weight ? (double)a.weight[row] : a.even;
-  int n;
-  const float part = frexpf(sum, &n);  // log sum: to 2^-25, whatever its size
-  const double logz = fma((double)n, 0.69314718055994531, (double)logf(part));
-  const double logp = bad ? (double)NAN : ((double)taken - (double)top) - logz;
+  const double logp = bad ? (double)NAN : ((double)taken - (double)top) - log_f64(sum);
   const double adv = a.adv[row], diff = logp - (double)a.old_logp[row];
-  const float ratio = expf((float)diff);
+  const Exp ratio = exp_f64(diff);
   const bool up = adv >= 0.0, clipped = up ? diff > a.log_high : diff < a.log_low;
   // the smaller of ratio adv and the clipped ratio's
-  const double gain = adv * (clipped ? (up ? 1.0 + (double)a.clip_high : 1.0 - (double)a.clip_low) : (double)ratio);
-  float kl = 0.f, dkl = 0.f;
+  const double gain = adv * (clipped ? (up ? 1.0 + (double)a.clip_high : 1.0 - (double)a.clip_low) : ratio.value);
+  double kl = 0.0, dkl = 0.0;
   if (a.ref_logp) {
-    const float gap = (float)((double)a.ref_logp[row] - logp);
-    kl = exp_rest(gap);
-    dkl = -expm1f(gap);
+    const double gap = (double)a.ref_logp[row] - logp;
+    const Exp e = exp_f64(gap);
+    kl = e.rest;
+    dkl = -e.less;
   }
   t.sums[0] = bad ? (double)NAN : w * ((double)a.kl_coef * kl - gain);
-  t.sums[1 + TALOS_POLICY_STAT_KL] = exp_rest((float)diff);  // (ratio - 1) - log ratio
+  t.sums[1 + TALOS_POLICY_STAT_KL] = ratio.rest;  // (ratio - 1) - log ratio
   t.sums[1 + TALOS_POLICY_STAT_POLICY] = gain;
   t.sums[1 + TALOS_POLICY_STAT_REF_KL] = kl;
   t.sums[1 + TALOS_POLICY_STAT_CLIPPED] = clipped ? 1.0 : 0.0;
   t.sums[1 + TALOS_POLICY_STAT_COUNT] = 1.0;
-  t.slope = bad ? 0.f : (float)(w * ((double)a.kl_coef * dkl - (clipped ? 0.0 : adv * ratio)));
+  t.slope = bad ? 0.f : (float)(w * ((double)a.kl_coef * dkl - (clipped ? 0.0 : adv * ratio.value)));
   t.logp = (float)logp;
   return t;
+}
+
+// The exponentials of a piece's values less the row's maximum, added up: fp32 ones and sums of a piece, as their roundings
+// average out over a long row (that of log2(e) itself, 1.3e-8 of every exponent, does not, and is put right); f64 ones in
+// rows of a few values (EXACT), where they do not.
+constexpr float kLog2e = 1.44269504f, kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e);
+template <bool EXACT, int N>
+__device__ __forceinline__ double exp_sum(const float (&v)[N], float top) {
+  if constexpr (EXACT) {
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += exp_f64((double)v[i] - (double)top).value;
+    return s;
+  } else {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float x = v[i] - top;
+      s += __builtin_amdgcn_exp2f(fmaf(x, kLog2e, x * kLog2eRest));
+    }
+    return (double)s;
+  }
+}
+__device__ __forceinline__ double lanes_sum_f64(double v, int lanes) {
+  for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+  return v;
 }
 
 // What a value adds to the sum of a lane or wave that has no maximum (every value -inf, or NaN): a NaN still shows.
@@ -99,13 +162,14 @@ __device__ __forceinline__ float none_or_nan(float v) { return v == -INFINITY ? 
 
 // One row per L lanes. V > 0: the row stays in registers, V pieces a lane; V = 0: any width, read again for the gradient
 // (L = 1024). dlogits null: the loss alone. dlogits may be the logits' own rows. (A workgroup that walks several rows
-// with the next one in flight holds the f64 functions' constants over the loop: 128 registers for 28, one workgroup a
-// compute unit for two, 131 -> 160 us at 4096 x 32768 bf16.)
+// with the next one in flight holds the f64 constants over the loop, one workgroup a compute unit for two: 131 -> 160 us
+// at 4096 x 32768 bf16.)
 template <typename T, int L, int V>
 __global__ __launch_bounds__(L > 256 ? L : 256) void policy_loss_kernel(PolicyArgs a, const T* logits, T* dlogits) {
   constexpr int N = Piece<T>::N, TB = L > 256 ? L : 256, R = TB / L, W = L > 64 ? L / 64 : 1;
   constexpr int LW = L < 64 ? L : 64;
-  __shared__ float tops[W], sums[W], slope_of[1];
+  __shared__ float tops[W], slope_of[1];
+  __shared__ double sums[W];
   __shared__ double part[R][kPolParts];
   const int lane = threadIdx.x % L, sub = threadIdx.x / L;
   const long long row = (long long)blockIdx.x * R + sub;
@@ -114,7 +178,8 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void policy_loss_kernel(PolicyAr
   const T* xr = logits + (in ? row : 0) * a.ld;
   T* dr = dlogits ? dlogits + (in ? row : 0) * a.ld_d : nullptr;
   if (lane < kPolParts) part[sub][lane] = 0.0;
-  float top = -INFINITY, sum = 0.f, slope = 0.f;
+  float top = -INFINITY, slope = 0.f;
+  double sum = 0.0;
   int act = -1;
   typename Piece<T>::Raw raw[V ? V : 1];
   if (on) {
@@ -123,7 +188,9 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void policy_loss_kernel(PolicyAr
     if constexpr (V > 0) {
       // values past the row are -inf: no maximum, no share of the sum
 #pragma unroll
-      for (int j = 0; j < V; ++j) raw[j] = load_raw(xr, N * (lane + L * j), a.vocab, -INFINITY);
+      for (int j = 0; j < V; ++j) raw[j] = row_piece(xr, N * (lane + L * j), a.vocab, -INFINITY);
+#pragma unroll
+      for (int j = 0; j < V; ++j) row_piece_end<T>(raw[j], N * (lane + L * j), a.vocab, -INFINITY);
       auto each = [&](auto&& f) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -141,14 +208,11 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void policy_loss_kernel(PolicyAr
       });
       top = lanes_max<LW>(top);
       if (top > -INFINITY) {
-        each([&](const float(&v)[N]) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) sum += __expf(v[i] - top);
-        });
+        each([&](const float(&v)[N]) { sum += exp_sum<(L < 64)>(v, top); });
       } else {
         each([&](const float(&v)[N]) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) sum += none_or_nan(v[i]);
+          for (int i = 0; i < N; ++i) sum += (double)none_or_nan(v[i]);
         });
       }
     } else {
@@ -163,24 +227,22 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void policy_loss_kernel(PolicyAr
 #pragma unroll
           for (int i = 0; i < N; ++i) most = fmaxf(most, v[u][i]);
         if (most > -INFINITY) {
-          sum *= __expf(top - most);
+          if (most > top) sum *= exp_f64((double)top - (double)most).value;
 #pragma unroll
-          for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < N; ++i) sum += __expf(v[u][i] - most);
+          for (int u = 0; u < U; ++u) sum += exp_sum<false>(v[u], most);
           top = most;
         } else {
 #pragma unroll
           for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum += none_or_nan(v[u][i]);
+            for (int i = 0; i < N; ++i) sum += (double)none_or_nan(v[u][i]);
         }
       }
       const float mine = top;
       top = lanes_max<LW>(top);
-      sum *= mine == -INFINITY ? 1.f : __expf(mine - top);
+      sum *= mine == -INFINITY ? 1.0 : exp_f64((double)mine - (double)top).value;
     }
-    sum = lanes_sum<LW>(sum);
+    sum = lanes_sum_f64(sum, LW);
     if constexpr (W > 1) {
       // the waves' maxima and sums, joined by every wave
       if ((threadIdx.x & 63) == 0) {
@@ -188,13 +250,14 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void policy_loss_kernel(PolicyAr
         sums[threadIdx.x >> 6] = sum;
       }
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < W; ++i) top = fmaxf(top, tops[i]);
-      sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < W; ++i) sum += sums[i] * (tops[i] == -INFINITY ? 1.f : __expf(tops[i] - top));
+      const int l64 = threadIdx.x & 63;
+      const float its = l64 < W ? tops[l64] : -INFINITY;
+      top = lanes_max<W>(its);
+      top = __shfl(top, 0, kWave);
+      sum = lanes_sum_f64(l64 < W ? sums[l64] * (its == -INFINITY ? 1.0 : exp_f64((double)its - (double)top).value) : 0.0, W);
+      sum = __shfl(sum, 0, kWave);
     }
-    if (top == -INFINITY) sum = NAN;  // no maximum in the whole row: no distribution
+    if (top == -INFINITY) sum = (double)NAN;  // no maximum in the whole row: no distribution
     // the row's scalars: one wave's work, not every wave's
     if (W == 1 || threadIdx.x < 64) {
       const RowTerms t = policy_row(a, (int)row, act < 0 || act >= a.vocab, top, sum, taken);
@@ -222,7 +285,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void policy_loss_kernel(PolicyAr
     }
   }
   if (!in || !dr) return;
-  const float scale = -slope / sum;
+  const float scale = -slope / (float)sum;
   auto grad = [&](float (&v)[N], int c) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -302,8 +365,8 @@ int policy_loss(const char* fn, int rows, int vocab, float clip_low, float clip_
   constexpr int N = Piece<T>::N;
   const int pieces = (vocab + N - 1) / N;
   PolicyArgs a{rows, vocab, clip_low, clip_high, kl_coef, std::log(std::max(0.0, 1.0 - (double)clip_low)),
-               std::log1p((double)clip_high), rows ? 1.0 / (double)rows : 0.0, ld, ld_d, actions, adv, old_logp, ref_logp, weight, logp,
-               nullptr};
+               std::log1p((double)clip_high), rows ? 1.0 / (double)rows : 0.0, ld, ld_d, actions, adv, old_logp,
+               ref_logp, weight, logp, nullptr};
   const int per = pieces <= 8 ? 32 : pieces <= 512 ? 4 : 1;  // rows a workgroup
   const int nblk = (int)ceil_div((size_t)rows, per);
   EntryScratch ws;

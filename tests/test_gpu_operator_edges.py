@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import operators_ref as ref
+import test_gpu_norm_loss as norm
 import talos_hip as th
 from operators_ref import float32_default  # noqa: F401
 
@@ -92,6 +93,34 @@ def test_layernorm_in_place(rows, dim, ty):
     th.call("talos_layernorm_fwd_" + ty, rows, dim, 1e-5, p(x), p(w), p(b), p(x), None, None, None)
     torch.cuda.synchronize()
     assert torch.equal(x, y) and torch.equal(dy, dx) and torch.equal(DW, want[0]) and torch.equal(DB, want[1])
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [2, 7, 9, 1540, 2055, 2056, 2057, 2304, 3100, 4100, 5001, 6143, 6145, 8191])
+def test_layernorm_where_shapes_change(dim, ty):
+    norm.test_layernorm(dim, ty)
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(53, 7573), (40, 23), (37, 40001), (700, 6)])
+def test_policy_loss_whose_gains_cancel(rows, vocab, ty):
+    """A loss of a thousandth of its terms, whose scalars are f64: what is left is the loss's own rounding and the errors of
+    the log-probabilities. In long rows an exponential is fp32, off by its own and its piece's roundings (2^-22) and its
+    argument's (2^-24 of it), which are independent: a row's sum is off by their root mean square, and the loss by that of
+    its rows. In short rows they are f64 (2^-38 is ample). Four deviations."""
+    x, a, adv, old, rp, w = norm.loss_inputs(rows, vocab, ty, 12)
+    loss0, *_ = ref.policy_loss(x.double(), a, adv.double(), old.double(), None, w.double(), 9.0, 9.0, 0.0)
+    lp = torch.log_softmax(x.double(), 1).gather(1, a.long()[:, None])[:, 0]
+    ratio = torch.exp(lp - old.double())
+    t = int((w * ratio).argmax())
+    adv[t] += float(loss0) / float(w[t].double() * ratio[t]) * 0.999  # the largest row balances the rest
+    loss, *_ = ref.policy_loss(x.double(), a, adv.double(), old.double(), None, w.double(), 9.0, 9.0, 0.0)
+    terms = (w.double() * ratio * adv.double()).abs()
+    assert abs(loss) < 0.1 * terms.sum()
+    got, *_ = norm.loss_call(ty, x, a, adv, old, None, w, (9.0, 9.0), 0.0)
+    gap = x.double() - x.double().max(1, keepdim=True).values
+    each = (torch.softmax(gap, 1) * (2.0 ** -22 - 2.0 ** -24 * gap)).norm(dim=1) if vocab > 64 else torch.tensor(2.0 ** -38)
+    assert abs(float(got) - loss) <= 2.0 ** -24 * abs(loss) + 4 * float((terms * each).norm())
 
 
 @pytest.mark.parametrize("ty", ["f32", "bf16"])
