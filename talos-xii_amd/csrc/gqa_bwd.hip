@@ -8,14 +8,15 @@
 //   dQ^T += K^T dS^T, with dS^T straight from the accumulator.
 // * dK and dV: a wave holds 32 keys and walks the queries of the group's heads, one head after the other:
 //   S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS. The heads of a group add into the same registers.
-// That is seven block products (eight for bf16, below) where one kernel that adds dQ atomically would need five.
+// That is seven block products where one kernel that adds dQ atomically would need five.
 //
 // D of a bf16 o. The forward's o carries the rounding of its probabilities and its own, 2^-9 of o each, and D from it is
-// off by that share of dO o: nothing to dQ and dK of long even rows, but of a row that sees few keys (or looks at few) o is
-// as large as v, and in dbias the error of a row meets the same distances again and again (2.7e-3 of dbias at 2 x 2048
-// tokens, where its fp32 sums are good to 1e-6). But sum_j dS_ij = 0 says what is missing: with D' from o, R_i =
-// sum_j p_ij (dP_ij - D'_i) is D - D', formed in fp32 beside the rest. The dQ kernel also sums p_ij k_j (one more block
-// product on the K tile's fragments in hand) and subtracts R times it; the dK / dV kernel, which runs after it, gets D' + R.
+// off by that share of dO o: of the size of dS's own rounding to bf16 in dQ and dK, but in dbias the error of a row meets
+// the same distances again and again (2.7e-3 of dbias at 2 x 2048 tokens, where its fp32 sums are good to 1e-6). But
+// sum_j dS_ij = 0 says what is missing: with D' from o, R_i = sum_j p_ij (dP_ij - D'_i) is D - D', formed in fp32 beside
+// the rest, and the dK / dV kernel, which runs after the dQ kernel, gets D' + R. dQ itself is summed with D': it is off
+// by 2.5e-3 for 2.4e-3 (4 x 4096 tokens, d 128), and R times sum_j p_ij k_j, which would put it right, is an eighth
+// block product that spills (fp32 registers: 256 and 66 spills for 216): 1770 us in all for 1580.
 //
 // The bias gradient belongs to the second kernel, where one head is at work: a block of 32 keys by 32 queries spans 63
 // distances. Blocks at least M away add into one register a lane; nearer ones sum their diagonals in registers
@@ -37,7 +38,7 @@ struct DqShape {
   static constexpr size_t lds = (size_t)NBUF * BUF * 2;
 };
 
-// waves a SIMD that the kernels are compiled for, as in the forward
+// waves a SIMD that the kernels are compiled for, as in the forward (which has the figures)
 template <typename T, int D, bool DMA>
 constexpr int kBwdWaves = D == 128 && !DMA ? 1 : 2;
 
@@ -120,14 +121,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
   }
 
   GqaLane<D> ln;
-  constexpr bool FIX = NP == 1;  // R and the sums of p k
-  gq_f32x16 acc[OB], pk[FIX ? OB : 1];
+  constexpr bool FIX = NP == 1;  // R is summed
+  gq_f32x16 acc[OB];
   float rest = 0.f;
 #pragma unroll
-  for (int i = 0; i < OB; ++i) {
-    acc[i] = gq_zero();
-    if (FIX) pk[i] = gq_zero();
-  }
+  for (int i = 0; i < OB; ++i) acc[i] = gq_zero();
 
   for (int t = t_beg; t < t_end; ++t) {
     uint16_t* buf = lds + (NBUF == 2 ? (t & 1) * S::BUF : 0);
@@ -201,28 +199,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
             dp[r] = 0.f;
           }
       }
-      float p[16], ds[16];
+      float ds[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, sub));
-        ds[r] = p[r] * (dp[r] - delta);
+        ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, sub)) * (dp[r] - delta);
         if (FIX) rest += ds[r];
       }
       const Frag<NP> df[2] = {gq_frag_acc<NP>(ds), gq_frag_acc<NP>(ds + 8)};
-      Frag<NP> pf[2];
-      if constexpr (FIX) {
-        pf[0] = gq_frag_acc<NP>(p);
-        pf[1] = gq_frag_acc<NP>(p + 8);
-      }
 #pragma unroll
       for (int i = 0; i < OB; ++i) {
         if constexpr (NP == 1) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const gq_bf16x8 f = gq_frag_tr<1, D, PL>(Kt, ln, 32 * kb + 16 * u, i).p[0];
-            acc[i] = gq_mfma(f, df[u].p[0], acc[i]);
-            pk[i] = gq_mfma(f, pf[u].p[0], pk[i]);
-          }
+          for (int u = 0; u < 2; ++u)
+            acc[i] = gq_mfma(gq_frag_tr<1, D, PL>(Kt, ln, 32 * kb + 16 * u, i).p[0], df[u].p[0], acc[i]);
         } else {
           gq_f32x16 x = gq_zero();
           Frag<NP> kf[2];
@@ -241,7 +230,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
   }
 
   if (qi >= a.Sq) return;
-  // one part: the result, and D for the next kernel. Parts: this one's sums (of p k too), R and D'.
+  // one part: the result, and D for the next kernel. Parts: this one's sums, R and D'.
   if (FIX) rest = gq_sum_halves(rest);
   const size_t rows = (size_t)a.B * a.H * a.Sq;
   if (h == 0 && (a.splits == 1 || it.split == 0)) a.delta[at] = a.splits == 1 ? delta + rest : delta;
@@ -254,27 +243,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
     for (int g4 = 0; g4 < 4; ++g4) {
       const int d = 32 * i + 8 * g4 + 4 * h;
       if (d >= a.dk) continue;
-      float x[4], y[4];
+      float x[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[j] = acc[i][4 * g4 + j];
-        if (FIX) {
-          y[j] = live ? pk[i][4 * g4 + j] : 0.f;
-          if (a.splits == 1) x[j] -= rest * y[j];
-        }
-        x[j] = live ? x[j] * a.scale : 0.f;
-      }
-      if (a.splits == 1) {
-        gq_store4(drow, d, a.dk, x);
-      } else {
-        gq_store4(a.part0 + prow * (FIX ? 2 : 1) * a.dk, d, a.dk, x);
-        if (FIX) gq_store4(a.part0 + (prow * 2 + 1) * a.dk, d, a.dk, y);
-      }
+      for (int j = 0; j < 4; ++j) x[j] = live ? acc[i][4 * g4 + j] * a.scale : 0.f;
+      if (a.splits == 1) gq_store4(drow, d, a.dk, x);
+      else gq_store4(a.part0 + prow * a.dk, d, a.dk, x);
     }
 }
 
-// The parts of dQ joined where R corrects it: 32 lanes a row. part0 [splits][B][Sq][H][scale sum dS' k | sum p k], part1
-// [splits][B][H][Sq] R; delta D' in, D out.
+// The parts of dQ and R joined: 32 lanes a row. part0 [splits][B][Sq][H][dk], part1 [splits][B][H][Sq]; delta D' in, D out.
 template <typename T>
 __global__ __launch_bounds__(256) void gqa_dq_join_kernel(GqaArgs a) {
   const long long rows = (long long)a.B * a.Sq * a.H, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -285,20 +262,14 @@ __global__ __launch_bounds__(256) void gqa_dq_join_kernel(GqaArgs a) {
   for (int s = 0; s < a.splits; ++s) rest += a.part1[s * rows + at];
   if (d == 0) a.delta[at] += rest;
   if (d >= a.dk) return;
-  float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
-    const float* p = a.part0 + (s * rows + row) * 2 * a.dk;
-    float v[4], w[4];
-    load_piece(p, d, a.dk, v);
-    load_piece(p + a.dk, d, a.dk, w);
+    float v[4];
+    load_piece(a.part0 + (s * rows + row) * a.dk, d, a.dk, v);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] += v[j];
-      y[j] += w[j];
-    }
+    for (int j = 0; j < 4; ++j) x[j] += v[j];
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] -= a.scale * rest * y[j];
   gq_store4(static_cast<T*>(a.dq) + token * a.lddq + (long long)head * a.dk, d, a.dk, x);
 }
 
@@ -652,19 +623,24 @@ BwdShape bwd_shape() {
            (const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 2, DMA>},
           DqShape<T, D, NK, NBK>::lds, DkvShape<T, D, NQ, NBQ>::lds};
 }
+// Tiles of keys (dQ) and of queries (dK, dV), two buffers each: 64 rows where a workgroup's LDS and registers hold them
+// beside a second workgroup's. Measured (forward and backward): 4 x 4096 tokens, d 128 bf16: query tiles of 64 1583 us, of
+// 32 1649; key tiles of 64 no better than 32 (1647). 2 x 2048, d 64 bf16: 276, with 32-row tiles 295. fp32, d 128, 21
+// samples of 1520 queries and 405 keys: two buffers of 32 rows 1595, one 1660. Direct tiles (gq_dma_fits): 4 x 4096, d 128
+// 1627 us, through registers 2260; 2 x 2048, d 64 276 and 278.
 template <typename T>
 BwdShape pick_bwd(int d, bool dma) {
   if constexpr (sizeof(T) == 2) {
     if (dma && d == 32) return bwd_shape<T, 32, 64, 2, 64, 2, true>();
     if (dma && d == 64) return bwd_shape<T, 64, 64, 2, 64, 2, true>();
-    if (dma && d == 128) return bwd_shape<T, 128, 32, 2, 32, 2, true>();
+    if (dma && d == 128) return bwd_shape<T, 128, 32, 2, 64, 2, true>();
     if (d <= 32) return bwd_shape<T, 32, 64, 2, 32, 2>();
     if (d <= 64) return bwd_shape<T, 64, 64, 2, 32, 2>();
     return bwd_shape<T, 128, 32, 2, 32, 2>();
   } else {
     if (d <= 32) return bwd_shape<T, 32, 32, 2, 32, 2>();
     if (d <= 64) return bwd_shape<T, 64, 32, 2, 32, 2>();
-    return bwd_shape<T, 128, 32, 1, 32, 1>();
+    return bwd_shape<T, 128, 32, 2, 32, 2>();
   }
 }
 
@@ -676,7 +652,9 @@ int launch(const void* fn, size_t blocks, size_t lds, GqaArgs* a, hipStream_t s,
 }
 
 constexpr int kDbiasMaxDistance = 512;  // four arrays of 2 M + 129 floats beside the tiles in a workgroup's LDS
-constexpr long long kFill = 512;  // workgroups that fill the device: two a compute unit
+// Workgroups that fill the device: two a compute unit (4 x 4096 tokens, d 128: 1627 us; for 256 1968, for 1024 1650; 2 x
+// 2048, d 64: 276, 277, 362).
+constexpr long long kFill = 512;
 
 template <typename T>
 int bwd(const char* fn, const talos_gqa_cfg* cfg, const int32_t* q_lens, const int32_t* k_lens, const float* bias,
@@ -712,7 +690,8 @@ int bwd(const char* fn, const talos_gqa_cfg* cfg, const int32_t* q_lens, const i
                    gq_dma_fits(dout, ld_do);
   const BwdShape shape = pick_bwd<T>(std::max(a.dk, a.dv), dma);
 
-  // parts of the key loop (dQ), of the heads and then of the query loop (dK, dV) where there is too little to do
+  // Parts of the key loop (dQ), of the heads and then of the query loop (dK, dV) where there is too little to do: of at
+  // least 256 keys or queries (22 samples of 247 queries and 79 keys, fp32 d 56: 168 us, with parts of 128 188).
   const long long pairs = (long long)a.B * a.KV;
   const long long q_tiles = ((long long)a.G * a.Sq + 127) / 128, k_tiles = (a.Sk + 127) / 128;
   const long long q_base = pairs * q_tiles, k_base = pairs * k_tiles;
@@ -720,7 +699,8 @@ int bwd(const char* fn, const talos_gqa_cfg* cfg, const int32_t* q_lens, const i
   long long sp_k = q_base ? std::min((fill + q_base - 1) / q_base, ((long long)a.Sk + 255) / 256) : 1;
   sp_k = std::max(1ll, sp_k);
   long long sp_h = 1, sp_q = 1;
-  // a causal key tile's share of the work, and a sample's, differ: twice the parts even them out
+  // a causal key tile's share of the work, and a sample's, differ: twice the parts even them out (4 x 4096, d 128: 1627 us,
+  // 1953 without)
   const long long fill_k = a.causal || q_lens || k_lens ? 2 * fill : fill;
   if (k_base && k_base < fill_k) {
     const long long want = (fill_k + k_base - 1) / k_base;
@@ -732,7 +712,7 @@ int bwd(const char* fn, const talos_gqa_cfg* cfg, const int32_t* q_lens, const i
     sp_q = std::max(1ll, std::min((want + sp_h - 1) / sp_h, ((long long)a.Sq + 255) / 256));
   }
   constexpr bool fix = sizeof(T) == 2;
-  const size_t dq_part = sp_k > 1 ? (size_t)sp_k * a.B * a.Sq * a.H * (fix ? 2 * a.dk + 1 : a.dk) : 0;
+  const size_t dq_part = sp_k > 1 ? (size_t)sp_k * a.B * a.Sq * a.H * (a.dk + (fix ? 1 : 0)) : 0;
   const size_t kv_part = sp_h * sp_q > 1 ? (size_t)(sp_h * sp_q) * a.B * a.Sk * a.KV * (a.dk + a.dv) : 0;
   const size_t n_delta = ((size_t)a.B * a.H * a.Sq + 63) & ~(size_t)63;
   const size_t n_bias = dbias && queries ? (size_t)a.B * a.H * k_tiles * sp_q * (2 * a.M + 1) : 0;
@@ -746,7 +726,7 @@ int bwd(const char* fn, const talos_gqa_cfg* cfg, const int32_t* q_lens, const i
     a.tiles = (int)q_tiles;
     a.splits = (int)sp_k;
     a.part0 = parts;
-    a.part1 = parts + (size_t)sp_k * a.B * a.Sq * a.H * 2 * a.dk;  // where R is kept
+    a.part1 = parts + (size_t)sp_k * a.B * a.Sq * a.H * a.dk;  // where R is kept
     rc = launch(shape.dq[bias ? 1 : 0], q_base * sp_k, shape.dq_lds, &a, s, "gqa_dq_kernel");
     if (!rc && sp_k > 1) {
       if constexpr (fix) {
