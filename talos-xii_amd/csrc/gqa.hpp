@@ -36,6 +36,7 @@ struct GqaArgs {
   float *lse, *delta;
   int tiles, splits;      // row tiles (or key tiles) a pair of sample and key head; parts a tile's loop is cut into
   float *part0, *part1;   // the parts' results where splits > 1: o or dq or dk, then lse or dv
+  int few;                // keys up to which a workgroup's dQ is corrected (bf16)
   int heads_per_split;    // dK / dV: splits = (G / heads_per_split) * splits_q
   int splits_q;
   float* dbias_part;      // [B][H][tiles][splits_q][2 M + 1]

@@ -11,12 +11,13 @@
 // That is seven block products where one kernel that adds dQ atomically would need five.
 //
 // D of a bf16 o. The forward's o carries the rounding of its probabilities and its own, 2^-9 of o each, and D from it is
-// off by that share of dO o: of the size of dS's own rounding to bf16 in dQ and dK, but in dbias the error of a row meets
-// the same distances again and again (2.7e-3 of dbias at 2 x 2048 tokens, where its fp32 sums are good to 1e-6). But
-// sum_j dS_ij = 0 says what is missing: with D' from o, R_i = sum_j p_ij (dP_ij - D'_i) is D - D', formed in fp32 beside
-// the rest, and the dK / dV kernel, which runs after the dQ kernel, gets D' + R. dQ itself is summed with D': it is off
-// by 2.5e-3 for 2.4e-3 (4 x 4096 tokens, d 128), and R times sum_j p_ij k_j, which would put it right, is an eighth
-// block product that spills (fp32 registers: 256 and 66 spills for 216): 1770 us in all for 1580.
+// off by that share of dO o: nothing beside dS's own rounding in rows that look at many keys, but of a row that sees few o
+// is as large as v (18 ragged tokens: error of dQ 3.1e-3 for 2.3e-3), and in dbias the error of a row meets the same
+// distances again and again (2.7e-3 of dbias at 2 x 2048 tokens, where its fp32 sums are good to 1e-6). But sum_j dS_ij = 0
+// says what is missing: with D' from o, R_i = sum_j p_ij (dP_ij - D'_i) is D - D', formed in fp32 beside the rest. The
+// dK / dV kernel, which runs after the dQ kernel, gets D' + R. dQ needs R times sum_j p_ij k_j as well, one more block
+// product, whose accumulators spill at d 128 (216 registers without it): workgroups of rows that see few keys run a kernel
+// with it, the others one without (4 x 4096 tokens, d 128, forward and backward 1459 us; all with it 1580).
 //
 // The bias gradient belongs to the second kernel, where one head is at work: a block of 32 keys by 32 queries spans 63
 // distances. Blocks at least M away add into one register a lane; nearer ones sum their diagonals in registers
@@ -24,6 +25,7 @@
 // additions meet, and the order is the program's. The four arrays are folded once a head. (Sixteen LDS float atomics a
 // block, each lane its values, cost 224 cycles apiece: 127 us of 322 at 2 x 2048 tokens, 16 heads, d 64, M 128.)
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "gqa.hpp"
@@ -42,9 +44,12 @@ struct DqShape {
 template <typename T, int D, bool DMA>
 constexpr int kBwdWaves = D == 128 && !DMA ? 1 : 2;
 
-// BIAS, DMA: as in the forward
-template <typename T, int D, int NK, int NBUF, bool BIAS, bool DMA>
+// BIAS, DMA: as in the forward. FIX (bf16): dQ is corrected by R, for the workgroups whose rows see at most a.few keys; the
+// others are the kernel's without it.
+template <typename T, int D, int NK, int NBUF, bool BIAS, bool DMA, bool FIX>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T, D, DMA>))) void gqa_dq_kernel(GqaArgs a) {
+  constexpr bool REST = sizeof(T) == 2;  // R is summed
+  static_assert(REST || !FIX, "fp32 rows have an exact D");
   using S = DqShape<T, D, NK, NBUF>;
   constexpr int NP = S::NP, KS = D / 16, OB = D / 32, KB = NK / 32, PL = NK * D;
   extern __shared__ __align__(16) uint16_t lds[];
@@ -61,6 +66,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
   const int lim_hi = q_lo >= sm.ql ? 0 : a.causal ? min(sm.kl, q_hi + sm.off + 1) : sm.kl;
   const int wg_lo = it.tile * S::ROWS / G, wg_hi = min((it.tile * S::ROWS + S::ROWS - 1) / G, sm.ql - 1);
   const int kend = wg_lo >= sm.ql ? 0 : a.causal ? max(0, min(sm.kl, wg_hi + sm.off + 1)) : sm.kl;
+  if (REST && FIX != (kend <= a.few)) return;
   const int ntile = (kend + NK - 1) / NK;
   const int t_beg = (int)((long long)ntile * it.split / a.splits), t_end = (int)((long long)ntile * (it.split + 1) / a.splits);
 
@@ -121,11 +127,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
   }
 
   GqaLane<D> ln;
-  constexpr bool FIX = NP == 1;  // R is summed
-  gq_f32x16 acc[OB];
+  gq_f32x16 acc[OB], pk[FIX ? OB : 1];
   float rest = 0.f;
 #pragma unroll
-  for (int i = 0; i < OB; ++i) acc[i] = gq_zero();
+  for (int i = 0; i < OB; ++i) {
+    acc[i] = gq_zero();
+    if (FIX) pk[i] = gq_zero();
+  }
 
   for (int t = t_beg; t < t_end; ++t) {
     uint16_t* buf = lds + (NBUF == 2 ? (t & 1) * S::BUF : 0);
@@ -199,19 +207,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
             dp[r] = 0.f;
           }
       }
-      float ds[16];
+      float p[16], ds[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, sub)) * (dp[r] - delta);
-        if (FIX) rest += ds[r];
+        p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, sub));
+        ds[r] = p[r] * (dp[r] - delta);
+        if (REST) rest += ds[r];
       }
       const Frag<NP> df[2] = {gq_frag_acc<NP>(ds), gq_frag_acc<NP>(ds + 8)};
+      Frag<NP> pf[2];
+      if constexpr (FIX) {
+        pf[0] = gq_frag_acc<NP>(p);
+        pf[1] = gq_frag_acc<NP>(p + 8);
+      }
 #pragma unroll
       for (int i = 0; i < OB; ++i) {
         if constexpr (NP == 1) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-            acc[i] = gq_mfma(gq_frag_tr<1, D, PL>(Kt, ln, 32 * kb + 16 * u, i).p[0], df[u].p[0], acc[i]);
+          for (int u = 0; u < 2; ++u) {
+            const gq_bf16x8 f = gq_frag_tr<1, D, PL>(Kt, ln, 32 * kb + 16 * u, i).p[0];
+            acc[i] = gq_mfma(f, df[u].p[0], acc[i]);
+            if constexpr (FIX) pk[i] = gq_mfma(f, pf[u].p[0], pk[i]);
+          }
         } else {
           gq_f32x16 x = gq_zero();
           Frag<NP> kf[2];
@@ -230,10 +247,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
   }
 
   if (qi >= a.Sq) return;
-  // one part: the result, and D for the next kernel. Parts: this one's sums, R and D'.
-  if (FIX) rest = gq_sum_halves(rest);
+  // one part: the result, and D for the next kernel. Parts: this one's sums (of p k too), R and D'.
+  constexpr bool PARTS = FIX || !REST;
+  if (REST) rest = gq_sum_halves(rest);
   const size_t rows = (size_t)a.B * a.H * a.Sq;
-  if (h == 0 && (a.splits == 1 || it.split == 0)) a.delta[at] = a.splits == 1 ? delta + rest : delta;
+  if (h == 0 && (!PARTS || a.splits == 1 || it.split == 0)) a.delta[at] = !PARTS || a.splits == 1 ? delta + rest : delta;
   if (FIX && h == 0 && a.splits > 1) a.part1[it.split * rows + at] = rest;
   T* drow = static_cast<T*>(a.dq) + ((long long)it.b * a.Sq + qi) * a.lddq + (long long)head * a.dk;
   const size_t prow = it.split * rows + ((size_t)it.b * a.Sq + qi) * a.H + head;
@@ -243,15 +261,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kBwdWaves<T
     for (int g4 = 0; g4 < 4; ++g4) {
       const int d = 32 * i + 8 * g4 + 4 * h;
       if (d >= a.dk) continue;
-      float x[4];
+      float x[4], y[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = live ? acc[i][4 * g4 + j] * a.scale : 0.f;
-      if (a.splits == 1) gq_store4(drow, d, a.dk, x);
-      else gq_store4(a.part0 + prow * a.dk, d, a.dk, x);
+      for (int j = 0; j < 4; ++j) {
+        x[j] = acc[i][4 * g4 + j];
+        if (FIX) {
+          y[j] = live ? pk[i][4 * g4 + j] : 0.f;
+          if (a.splits == 1) x[j] -= rest * y[j];
+        }
+        x[j] = live ? x[j] * a.scale : 0.f;
+      }
+      if (!PARTS || a.splits == 1) {
+        gq_store4(drow, d, a.dk, x);
+      } else {
+        gq_store4(a.part0 + prow * (FIX ? 2 : 1) * a.dk, d, a.dk, x);
+        if (FIX) gq_store4(a.part0 + (prow * 2 + 1) * a.dk, d, a.dk, y);
+      }
     }
 }
 
-// The parts of dQ and R joined: 32 lanes a row. part0 [splits][B][Sq][H][dk], part1 [splits][B][H][Sq]; delta D' in, D out.
+// The parts of dQ joined where R corrects it: 32 lanes a row. part0 [splits][B][Sq][H][scale sum dS' k | sum p k], part1
+// [splits][B][H][Sq] R; delta D' in, D out.
 template <typename T>
 __global__ __launch_bounds__(256) void gqa_dq_join_kernel(GqaArgs a) {
   const long long rows = (long long)a.B * a.Sq * a.H, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -259,17 +289,25 @@ __global__ __launch_bounds__(256) void gqa_dq_join_kernel(GqaArgs a) {
   const int d = 4 * (threadIdx.x & 31), head = (int)(row % a.H);
   const long long token = row / a.H, at = (token / a.Sq * a.H + head) * a.Sq + token % a.Sq;
   float rest = 0.f;
+#pragma unroll 4
   for (int s = 0; s < a.splits; ++s) rest += a.part1[s * rows + at];
   if (d == 0) a.delta[at] += rest;
   if (d >= a.dk) return;
-  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
-    float v[4];
-    load_piece(a.part0 + (s * rows + row) * a.dk, d, a.dk, v);
+    const float* p = a.part0 + (s * rows + row) * 2 * a.dk;
+    float v[4], w[4];
+    load_piece(p, d, a.dk, v);
+    load_piece(p + a.dk, d, a.dk, w);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] += v[j];
+    for (int j = 0; j < 4; ++j) {
+      x[j] += v[j];
+      y[j] += w[j];
+    }
   }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] -= a.scale * rest * y[j];
   gq_store4(static_cast<T*>(a.dq) + token * a.lddq + (long long)head * a.dk, d, a.dk, x);
 }
 
@@ -611,14 +649,21 @@ __global__ __launch_bounds__(1024) void gqa_dbias_kernel(int B, int H, int per, 
 
 // The kernels of one head width.
 struct BwdShape {
-  const void* dq[2];
+  const void *dq[2], *dq_few[2];  // dq_few: null for fp32
   const void* dkv[3];
   size_t dq_lds;
   size_t (*dkv_lds)(bool, int);
 };
 template <typename T, int D, int NK, int NBK, int NQ, int NBQ, bool DMA = false>
 BwdShape bwd_shape() {
-  return {{(const void*)gqa_dq_kernel<T, D, NK, NBK, false, DMA>, (const void*)gqa_dq_kernel<T, D, NK, NBK, true, DMA>},
+  const void *few = nullptr, *few_bias = nullptr;
+  if constexpr (sizeof(T) == 2) {
+    few = (const void*)gqa_dq_kernel<T, D, NK, NBK, false, DMA, true>;
+    few_bias = (const void*)gqa_dq_kernel<T, D, NK, NBK, true, DMA, true>;
+  }
+  return {{(const void*)gqa_dq_kernel<T, D, NK, NBK, false, DMA, false>,
+           (const void*)gqa_dq_kernel<T, D, NK, NBK, true, DMA, false>},
+          {few, few_bias},
           {(const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 0, DMA>, (const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 1, DMA>,
            (const void*)gqa_dkv_kernel<T, D, NQ, NBQ, 2, DMA>},
           DqShape<T, D, NK, NBK>::lds, DkvShape<T, D, NQ, NBQ>::lds};
@@ -651,6 +696,10 @@ int launch(const void* fn, size_t blocks, size_t lds, GqaArgs* a, hipStream_t s,
   return hip_status(hipLaunchKernel(fn, dim3((unsigned)blocks), dim3(256), args, lds, s), name);
 }
 
+// Keys up to which a workgroup of bf16 rows has its dQ corrected by R. The error of dQ, 4 x 4096 causal tokens: 2.36e-3 with
+// any of 64 to 512 (2.45e-3 uncorrected), 672 ragged ones 2.35e-3 (2.52e-3), 3799 queries of 781 keys 2.39e-3 with 64 or 128,
+// 2.37e-3 with 256; time of the first 1447, 1459, 1467, 1476 us for 64, 128, 256, 512.
+constexpr int kFewKeys = 128;
 constexpr int kDbiasMaxDistance = 512;  // four arrays of 2 M + 129 floats beside the tiles in a workgroup's LDS
 // Workgroups that fill the device: two a compute unit (4 x 4096 tokens, d 128: 1627 us; for 256 1968, for 1024 1650; 2 x
 // 2048, d 64: 276, 277, 362).
@@ -712,7 +761,7 @@ int bwd(const char* fn, const talos_gqa_cfg* cfg, const int32_t* q_lens, const i
     sp_q = std::max(1ll, std::min((want + sp_h - 1) / sp_h, ((long long)a.Sq + 255) / 256));
   }
   constexpr bool fix = sizeof(T) == 2;
-  const size_t dq_part = sp_k > 1 ? (size_t)sp_k * a.B * a.Sq * a.H * (a.dk + (fix ? 1 : 0)) : 0;
+  const size_t dq_part = sp_k > 1 ? (size_t)sp_k * a.B * a.Sq * a.H * (fix ? 2 * a.dk + 1 : a.dk) : 0;
   const size_t kv_part = sp_h * sp_q > 1 ? (size_t)(sp_h * sp_q) * a.B * a.Sk * a.KV * (a.dk + a.dv) : 0;
   const size_t n_delta = ((size_t)a.B * a.H * a.Sq + 63) & ~(size_t)63;
   const size_t n_bias = dbias && queries ? (size_t)a.B * a.H * k_tiles * sp_q * (2 * a.M + 1) : 0;
@@ -726,8 +775,12 @@ int bwd(const char* fn, const talos_gqa_cfg* cfg, const int32_t* q_lens, const i
     a.tiles = (int)q_tiles;
     a.splits = (int)sp_k;
     a.part0 = parts;
-    a.part1 = parts + (size_t)sp_k * a.B * a.Sq * a.H * a.dk;  // where R is kept
-    rc = launch(shape.dq[bias ? 1 : 0], q_base * sp_k, shape.dq_lds, &a, s, "gqa_dq_kernel");
+    a.part1 = parts + (size_t)sp_k * a.B * a.Sq * a.H * 2 * a.dk;  // where R is kept
+    // fp32, or bf16 workgroups by the keys that their rows see (those with parts are few and see little each)
+    a.few = sp_k > 1 ? INT_MAX : kFewKeys;
+    const bool some = !fix || a.Sk > a.few, few = fix && (!some || a.causal || q_lens || k_lens);
+    if (some) rc = launch(shape.dq[bias ? 1 : 0], q_base * sp_k, shape.dq_lds, &a, s, "gqa_dq_kernel");
+    if (!rc && few) rc = launch(shape.dq_few[bias ? 1 : 0], q_base * sp_k, shape.dq_lds, &a, s, "gqa_dq_kernel");
     if (!rc && sp_k > 1) {
       if constexpr (fix) {
         hipLaunchKernelGGL(gqa_dq_join_kernel<T>, dim3(ceil_div((size_t)a.B * a.Sq * a.H, 8)), dim3(256), 0, s, a);

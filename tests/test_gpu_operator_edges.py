@@ -171,3 +171,46 @@ def test_two_streams_at_once(ty):
     finally:
         for s in streams:
             th.stream_destroy(s)
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+def test_wide_heads_in_a_graph(ty):
+    """Head dims of 128, whose tiles take more than 64 KB of a workgroup's LDS, captured; eager work between the replays."""
+    B, S, H, KV, d, M = 2, 190, 4, 2, 128, 33
+    g = torch.Generator(device="cuda").manual_seed(6)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").to(DT[ty])  # noqa: E731
+    q, k, v, do = rnd(B, S, H, d), rnd(B, S, KV, d), rnd(B, S, KV, d), rnd(B, S, H, d)
+    bias = torch.randn(H, 2 * M + 1, generator=g, device="cuda")
+    out = [torch.zeros_like(t) for t in (do, q, k, v, bias)] + [torch.zeros(B, H, S, device="cuda")]
+    o, dq, dk, dv, db, lse = out
+    cfg = th.GqaCfg(B, S, S, H, KV, d, d, 1, M, d ** -0.5)
+
+    def go(s):
+        ins = [None, None, p(bias), p(q), H * d, p(k), KV * d, p(v), KV * d, p(o), H * d, p(lse)]
+        th.call("talos_gqa_fwd_" + ty, cfg, *ins, s)
+        th.call("talos_gqa_bwd_" + ty, cfg, *ins, p(do), H * d, p(dq), H * d, p(dk), KV * d, p(dv), KV * d, 0.0, p(db), s)
+
+    keep = torch.empty(32 << 20, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    stream = th.stream_create()
+    th.call("talos_workspace_bind", keep.data_ptr(), keep.numel())
+    try:
+        graph = th.Graph(stream, lambda: go(stream))
+        want = None
+        for turn in range(3):
+            for t in out:
+                t.zero_()
+            torch.cuda.synchronize()
+            go(None)
+            torch.cuda.synchronize()
+            want = [t.clone() for t in out]
+            for t in out:
+                t.fill_(7.0)
+            torch.cuda.synchronize()
+            graph.launch()
+            th.call("talos_stream_sync", stream)
+            for t, w in zip(out, want):
+                assert torch.equal(t, w), turn
+    finally:
+        th.call("talos_workspace_bind", None, 0)
+        th.stream_destroy(stream)
