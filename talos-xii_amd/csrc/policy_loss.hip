@@ -12,8 +12,7 @@
 // the registers), its maximum, its sum of exponentials and the taken logit are formed, and the gradient
 // is written from the same registers: one read and one write of the logits for loss and gradient
 // together. L lanes hold a row, V pieces each: 8 lanes up to 32 (fp32) or 64 (bf16) actions, a wave
-// up to 2048 or 4096, four waves or sixteen beyond, up to 16384 fp32 or 32768 bf16 columns; wider rows are
-// read again. The
+// up to 2048 or 4096, four waves or eight beyond, up to 32768 columns; wider rows are read again. The
 // exponentials are fp32 (f64 in rows of a few values), their sums f64 from a piece on.
 //
 // Rows of weight 0 are padding: their logits are not read, their gradient is zero.
@@ -28,10 +27,13 @@ namespace {
 
 // partial sums of a workgroup: the loss, then the entries of enum talos_policy_stat
 constexpr int kPolParts = 1 + TALOS_POLICY_NSTATS;
-// 16-byte pieces of a row that sixteen waves hold (4 a lane). With 8 a lane a compute unit no longer has room for two
-// workgroups, and reading the row again, from cache, is faster: 2048 x 30001 fp32 138 -> 130 us, x 40000 bf16 114 -> 83;
-// with 4, holding is: 4096 x 32768 bf16 136 -> 117 us.
-constexpr int kHeld = 4096;
+// 16-byte pieces of a row that eight waves hold, 8 or (fp32) 16 a lane; a wider row is read again, from cache. Eight waves
+// leave room for other rows at other phases: 4096 x 20001 bf16 97 us, with sixteen of half the pieces 109; 4096 x 32768 115
+// and 117, reading again 136. 16 a lane hold fp32 rows of twice as many pieces (2048 x 30001 110 us, 134 reading again; x
+// 20000 75 and 85); of bf16 rows, twice as many values, they gain near the full width alone (x 60000 126 and 136, x 40000
+// 95 and 89).
+template <typename T>
+constexpr int kHeld = sizeof(T) == 4 ? 8192 : 4096;
 constexpr int kPolicyMaxVocab = 1 << 26;
 
 struct PolicyArgs {
@@ -376,14 +378,15 @@ int policy_loss(const char* fn, int rows, int vocab, float clip_low, float clip_
   if (nblk > 0) {
 #define TALOS_POL(L, V)                                                                                          \
   hipLaunchKernelGGL((policy_loss_kernel<T, L, V>), dim3(nblk), dim3(L > 256 ? L : 256), 0, s, a, logits, dlogits)
-    if (pieces > kHeld) TALOS_POL(1024, 0);
+    if (pieces > kHeld<T>) TALOS_POL(1024, 0);
     else if (pieces <= 8) TALOS_POL(8, 1);
     else if (pieces <= 64) TALOS_POL(64, 1);
     else if (pieces <= 256) TALOS_POL(64, 4);
     else if (pieces <= 512) TALOS_POL(64, 8);
     else if (pieces <= 1024) TALOS_POL(256, 4);
     else if (pieces <= 2048) TALOS_POL(256, 8);
-    else TALOS_POL(1024, 4);
+    else if (pieces <= 4096) TALOS_POL(512, 8);
+    else if constexpr (sizeof(T) == 4) TALOS_POL(512, 16);
 #undef TALOS_POL
     rc = launch_status("policy_loss_kernel");
   }
